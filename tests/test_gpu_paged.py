@@ -1,0 +1,587 @@
+"""GPU tests of the paged key-value cache (include/tq4_paged.h, transmuter_b200.paged) against the
+float64 oracle (oracle/paged.py).
+
+Tolerances: a 16-bit output is off by at most half a step of its type (torch.finfo(t).eps / 2 relative)
+beyond the oracle's bound of a 32-bit evaluation; an attention over a 16-bit cache also rounds each
+softmax weight once to that type before it multiplies the values, half a step of each weight more.
+Cache rows outside the sequences hold NaN throughout, so that a row read too many shows.
+"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged as po
+from transmuter_b200 import _lib, paged
+from transmuter_b200.deferred import ArgumentError
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+BAD = 0x200
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def f64(x):
+    return x.detach().double().cpu().numpy()
+
+
+def device_status():
+    import ctypes
+    code = ctypes.c_int32()
+    _lib.check(_lib.load().tq4_device_status(0, ctypes.byref(code)))
+    return code.value
+
+
+@pytest.fixture(autouse=True)
+def clean_status():
+    device_status()
+    yield
+    assert device_status() == 0, "a device-side check fired"
+
+
+def make_pool(lengths, kv, ps, d, dtype, seed=0, spare=3, width=None, fresh=0):
+    """Shuffled pages whose rows in use are normal and whose others are NaN; `fresh` unlisted pages a
+    sequence in a second table."""
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-n // ps) for n in lengths]
+    total = sum(need) + spare + fresh * len(lengths)
+    order = torch.randperm(total, generator=g).int()
+    width = width or max(need + [1])
+    table = torch.full((len(lengths), width), -1, dtype=torch.int32)
+    k = torch.full((total, kv, ps, d), math.nan)
+    v = torch.full((total, kv, ps, d), math.nan)
+    at = 0
+    for s, n in enumerate(lengths):
+        table[s, :need[s]] = order[at:at + need[s]]
+        at += need[s]
+        for j in range(n):
+            k[table[s, j // ps], :, j % ps] = torch.randn(kv, d, generator=g)
+            v[table[s, j // ps], :, j % ps] = torch.randn(kv, d, generator=g)
+    new = order[at:at + fresh * len(lengths)].reshape(len(lengths), fresh).to(DEV)
+    return k.to(DEV, dtype), v.to(DEV, dtype), table.to(DEV), new
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+# ---- append -----------------------------------------------------------------------------------
+
+APPENDS = [
+    # dtype, heads, kv, d, page, pairs, axes, interleaved, norm
+    (F32, 16, 8, 128, 16, 64, 1, False, True),
+    (BF16, 32, 8, 128, 16, 64, 1, False, False),
+    (BF16, 28, 4, 128, 32, 64, 3, False, True),
+    (F16, 6, 2, 80, 8, 40, 3, True, True),
+    (F16, 3, 3, 72, 1, 36, 1, False, True),
+    (F32, 5, 1, 12, 2, 3, 2, True, False),
+    (BF16, 4, 2, 256, 16, 64, 4, False, True),
+    (F32, 4, 2, 256, 64, 128, 1, True, True),
+    (F16, 2, 1, 8, 4, 4, 1, False, False),
+    (F16, 2, 1, 40, 4, 0, 1, False, True),
+    (BF16, 40, 2, 64, 16, 10, 1, True, False),
+]
+
+
+def run_append(dtype, heads, kv, d, ps, pairs, axes, interleaved, norm, tokens=7, strided=True, offset=0, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    max_pos = 50
+    lengths = [5, 0, 20]
+    k_pages, v_pages, table, _ = make_pool([9, 4, 30], kv, ps, d, dtype, seed)
+    seq = [s for _, s in zip(range(tokens), [0, 2, 1, 2, 0, 2, 1] * 10)]
+    slot = []
+    for s in seq:  # the next free slot of each sequence
+        slot.append(lengths[s])
+        lengths[s] += 1
+    width = (heads + 2 * kv) * d
+    qkv = torch.randn(tokens + 1, width + (5 if strided else 0) + offset, generator=g).to(DEV, dtype)[:tokens]
+    row = qkv[:, offset:offset + width]
+    q, k, v = (x.unflatten(1, (-1, d)) for x in (row[:, :heads * d], row[:, heads * d:(heads + kv) * d], row[:, (heads + kv) * d:]))
+    positions = torch.randint(0, max_pos, (axes, tokens), generator=g).int().to(DEV)
+    ang = torch.randn(max_pos, pairs, generator=g)
+    pair_axis = [i % axes for i in range(pairs)]
+    w = [torch.rand(d, generator=g).add(0.5).to(DEV) if norm else None for _ in range(2)]
+    rot = paged.Rotary(ang.cos().to(DEV), ang.sin().to(DEV), pair_axis=pair_axis, interleaved=interleaved, q_weight=w[0],
+                       k_weight=w[1], eps=1e-6)
+    rot.axes, rot._desc.axes = axes, axes  # also where the last axes have no pair
+    cache = paged.PagedCache(k_pages, v_pages, table)
+    want_k, want_v = f64(k_pages), f64(v_pages)
+    out = cache.append(q, k, v, ints(seq), ints(slot), positions, rot)
+    torch.cuda.synchronize()
+    got_k, got_v, got_q = f64(k_pages), f64(v_pages), f64(out)
+    eps = half_step(dtype) if dtype != F32 else 0.0
+    tiny = 2.0 ** -25 if dtype == F16 else 0.0  # half of f16's subnormal step
+    args = (1e-6, f64(ang.cos()), f64(ang.sin()), pair_axis)
+    pos, tab = positions.cpu().numpy(), table.cpu().numpy()
+
+    def check(got, x, wt, t):
+        y, bound = po.norm_rotate(f64(x), None if wt is None else f64(wt), *args, pos[:, t], interleaved)
+        assert np.all(np.abs(got - y) <= bound * (1 + eps) + np.abs(y) * eps + tiny)
+
+    for t in range(tokens):
+        for h in range(heads):
+            check(got_q[t, h], q[t, h], w[0], t)
+        page, r = po.place(tab, ps, seq[t], slot[t])
+        for h in range(kv):
+            check(got_k[page, h, r], k[t, h], w[1], t)
+            want_k[page, h, r] = got_k[page, h, r]
+            want_v[page, h, r] = f64(v[t, h])
+    # every other row is as it was, and values are copied bit for bit
+    assert np.array_equal(got_k, want_k, equal_nan=True) and np.array_equal(got_v, want_v, equal_nan=True)
+
+
+@pytest.mark.parametrize("case", APPENDS, ids=str)
+def test_append(case):
+    run_append(*case)
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 33])
+@pytest.mark.parametrize("case", [APPENDS[0], APPENDS[2]], ids=str)
+def test_append_token_counts(case, tokens):
+    run_append(*case, tokens=tokens if tokens < 33 else 12, strided=tokens == 2)
+
+
+@pytest.mark.parametrize("offset", [1, 2, 8])
+def test_append_reads_unaligned_views(offset):
+    run_append(BF16, 4, 2, 64, 16, 32, 1, False, True, offset=offset)
+
+
+def simple_cache(dtype=BF16, lengths=(5, 3), kv=2, ps=4, d=64, width=None):
+    k, v, table, _ = make_pool(list(lengths), kv, ps, d, dtype, 3, width=width)
+    return paged.PagedCache(k, v, table)
+
+
+def test_append_without_queries_fills_the_cache():
+    c = simple_cache()
+    k, v = torch.randn(2, 3, 2, 64, device=DEV).to(BF16)
+    assert c.append(None, k, v, ints([0, 1, 1]), ints([4, 0, 2])) is None
+    for t, (s, j) in enumerate([(0, 4), (1, 0), (1, 2)]):
+        p = c.page_table[s, j // 4]
+        assert torch.equal(c.k_pages[p, :, j % 4], k[t]) and torch.equal(c.v_pages[p, :, j % 4], v[t])
+
+
+def test_append_leaves_padding_alone():
+    c = simple_cache()
+    q, out = torch.randn(3, 4, 64, device=DEV).to(BF16), torch.full((3, 4, 64), 7.0, device=DEV, dtype=BF16)
+    k, v = torch.randn(2, 3, 2, 64, device=DEV).to(BF16)
+    before = c.k_pages.clone(), c.v_pages.clone()
+    c.append(q, k, v, ints([-1, 0, -1]), ints([0, 1, -5]), out=out)
+    assert torch.equal(out[1], q[1]) and (out[0] == 7).all() and (out[2] == 7).all()
+    p = c.page_table[0, 0]
+    before[0][p, :, 1], before[1][p, :, 1] = k[1], v[1]
+    assert torch.equal(c.k_pages.nan_to_num(9), before[0].nan_to_num(9))
+    assert torch.equal(c.v_pages.nan_to_num(9), before[1].nan_to_num(9))
+
+
+@pytest.mark.parametrize("seq,slot,pos", [(2, 0, 0), (0, 8, 0), (0, -1, 0), (0, 0, 20), (0, 0, -1), (1, 7, 0)])
+def test_append_flags_what_is_out_of_range(seq, slot, pos):
+    c = simple_cache(width=2)  # sequence 1 has no second page: its entry is -1
+    q, out = torch.randn(1, 4, 64, device=DEV).to(BF16), torch.zeros(1, 4, 64, device=DEV, dtype=BF16)
+    k, v = torch.randn(2, 1, 2, 64, device=DEV).to(BF16)
+    ang = torch.randn(20, 32, device=DEV)
+    before = c.k_pages.nan_to_num(9), c.v_pages.nan_to_num(9)
+    c.append(q, k, v, ints([seq]), ints([slot]), ints([pos]), paged.Rotary(ang.cos(), ang.sin()), out=out)
+    assert device_status() == BAD
+    assert torch.equal(c.k_pages.nan_to_num(9), before[0]) and torch.equal(c.v_pages.nan_to_num(9), before[1])
+    assert not out.any()
+
+
+# ---- attention --------------------------------------------------------------------------------
+
+ATTENTIONS = [
+    # dtype, heads, kv, d, page, lengths, window, scores
+    (F32, 16, 8, 128, 16, [257], 0, False),
+    (BF16, 32, 8, 128, 16, [1, 0, 15, 16, 17, 100, 333], 0, True),
+    (F16, 32, 8, 128, 64, [1000, 3], 0, True),
+    (F16, 28, 4, 80, 16, [300, 0, 31, 32, 33], 100, True),
+    (F32, 8, 8, 64, 32, [63, 64, 65, 1], 0, True),
+    (BF16, 8, 1, 256, 8, [130, 7], 0, True),
+    (F32, 6, 2, 256, 8, [70], 3, True),
+    (F16, 20, 1, 72, 1, [40, 5], 0, True),
+    (BF16, 32, 2, 40, 128, [200, 129], 1, True),
+    (F16, 2, 2, 8, 2, [19, 1], 0, False),
+    (F32, 3, 1, 12, 4, [37, 0, 0], 36, True),
+    (BF16, 15, 3, 96, 16, [90, 500], 500, False),
+    (F32, 16, 1, 64, 16, [200], 0, True),
+    (BF16, 17, 1, 64, 16, [77], 0, True),
+    (BF16, 64, 1, 128, 16, [160], 0, True),
+]
+
+
+def check_attention(out, new, c, q, lengths, window, scores, scale=None):
+    dtype = c.dtype
+    scale = 1 / math.sqrt(c.head_dim) if scale is None else scale
+    k, v = f64(c.k_pages), f64(c.v_pages)
+    want, bound, want_new, new_bound = po.attention(f64(q), k, v, c.page_table.cpu().numpy(), lengths, scale, window,
+                                                    None if scores is None else f64(scores))
+    tol = bound
+    if dtype != F32:
+        mean_abs = po.attention(f64(q), k, np.abs(v), c.page_table.cpu().numpy(), lengths, scale, window)[0]
+        tol = bound + half_step(dtype) * (mean_abs + np.abs(want)) + (2.0 ** -24 if dtype == F16 else 0.0)
+    else:
+        tol = tol + np.abs(want) * po.U
+    got = f64(out)
+    assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) - tol)
+    if scores is not None:
+        assert np.all(np.abs(f64(new) - want_new) <= new_bound), np.max(np.abs(f64(new) - want_new) - new_bound)
+
+
+def run_attention(dtype, heads, kv, d, ps, lengths, window, with_scores, seed=2, gain=2.0, scale=None):
+    k, v, table, _ = make_pool(lengths, kv, ps, d, dtype, seed, width=-(-max(lengths) // ps) + 2)
+    c = paged.PagedCache(k, v, table)
+    g = torch.Generator(DEV).manual_seed(seed)
+    q = (torch.randn(len(lengths), heads, d, device=DEV, generator=g) * gain).to(dtype)
+    scores = torch.rand(len(lengths), kv, c.max_slots, device=DEV, generator=g) if with_scores else None
+    new = torch.full_like(scores, -7.0) if with_scores else None
+    out = c.attention(q, ints(lengths), scale=scale, window=window, scores=scores, new_scores=new)
+    if with_scores:  # behind each sequence nothing is written
+        for b, n in enumerate(lengths):
+            assert (new[b, :, n:] == -7).all()
+            new[b, :, n:] = scores[b, :, n:]
+    check_attention(out, new, c, q, lengths, window, scores, scale)
+    return c, q, out
+
+
+@pytest.mark.parametrize("case", ATTENTIONS, ids=str)
+def test_attention(case):
+    run_attention(*case)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("gain,scale", [(40.0, None), (1.0, 0.0), (2.0, -0.3), (1e-3, 2.0)])
+def test_attention_scales(dtype, gain, scale):
+    run_attention(dtype, 8, 2, 64, 16, [100, 1, 33], 0, True, gain=gain, scale=scale)
+
+
+@pytest.mark.parametrize("dtype,heads", [(F32, 4), (BF16, 4), (F16, 32)])
+def test_attention_many_sequences(dtype, heads):
+    lengths = [(i * 37) % 61 for i in range(700)]  # more rows than CTAs, some empty
+    run_attention(dtype, heads, 2, 16, 4, lengths, 0, True)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_attention_in_place_scores_and_strided_queries(dtype):
+    lengths, kv, d = [50, 20], 2, 64
+    k, v, table, _ = make_pool(lengths, kv, 16, d, dtype, 5)
+    c = paged.PagedCache(k, v, table)
+    wide = torch.randn(2, 500, device=DEV).to(dtype)
+    q = wide[:, 3:3 + 4 * d].unflatten(1, (4, d))
+    scores = torch.rand(2, kv, c.max_slots, device=DEV)
+    old = scores.clone()
+    a = c.attention(q, ints(lengths))
+    b = c.attention(q, ints(lengths), scores=scores)
+    assert torch.equal(a, b)
+    check_attention(b, scores, c, q, lengths, 0, old)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_is_deterministic_and_independent_of_the_workspace(dtype):
+    lengths = [1500, 3, 700]
+    k, v, table, _ = make_pool(lengths, 2, 16, 128, dtype, 6)
+    c = paged.PagedCache(k, v, table)
+    q = torch.randn(3, 8, 128, device=DEV).to(dtype)
+    first = c.attention(q, ints(lengths))
+    n = c._workspace[(8, 3, False)]
+    junk = torch.full((n,), 0xFF, dtype=torch.uint8, device=DEV)  # NaN wherever a float is read unwritten
+    del junk
+    for _ in range(3):
+        assert torch.equal(c.attention(q, ints(lengths)), first)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_attention_shared_prefix_pages(dtype):
+    k, v, table, _ = make_pool([40, 40], 2, 16, 64, dtype, 7)
+    table[1, 0] = table[0, 0]
+    c = paged.PagedCache(k, v, table)
+    q = torch.randn(2, 4, 64, device=DEV).to(dtype)
+    check_attention(c.attention(q, ints([40, 33])), None, c, q, [40, 33], 0, None)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_flags_bad_lengths_and_pages(dtype):
+    k, v, table, _ = make_pool([20, 20, 20, 20], 2, 4, 64, dtype, 8)
+    c = paged.PagedCache(k, v, table)
+    q = torch.randn(4, 4, 64, device=DEV).to(dtype)
+    good = c.attention(q, ints([20, 20, 20, 20]))
+    out = c.attention(q, ints([20, -1, c.max_slots + 1, 20]))
+    assert device_status() == BAD
+    assert torch.equal(out[0], good[0]) and torch.equal(out[3], good[3]) and not out[1:3].any()
+    table[1, 2], table[2, 2] = c.num_pages, -1  # slots 8 to 11 of these are left out
+    out = c.attention(q, ints([20, 20, 20, 20]))
+    assert device_status() == BAD
+    assert torch.equal(out[0], good[0]) and torch.equal(out[3], good[3])
+    rest = paged.PagedCache(k, v, torch.cat([table[:, :2], table[:, 3:]], 1).contiguous())
+    check_attention(out[1:3], None, rest_rows(rest, 1, 3), q[1:3], [16, 16], 0, None)
+
+
+def rest_rows(c, lo, hi):
+    return paged.PagedCache(c.k_pages, c.v_pages, c.page_table[lo:hi].contiguous())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_attention_infinite_values_stay_in_their_rows(dtype):
+    """An infinite or NaN value in one sequence reaches no other."""
+    k, v, table, _ = make_pool([30, 30], 1, 16, 64, dtype, 9)
+    c = paged.PagedCache(k, v, table)
+    q = torch.randn(2, 2, 64, device=DEV).to(dtype)
+    good = c.attention(q, ints([30, 30]))
+    v[table[0, 1], 0, 3, 5] = math.inf
+    k[table[0, 0], 0, 3] = math.nan
+    out = c.attention(q, ints([30, 30]))
+    assert torch.equal(out[1], good[1]) and out[0].isnan().any()
+
+
+def test_attention_past_2_31_values():
+    """Pages beyond 2^31 values from the pool's start, and a sequence beyond 2^16 slots."""
+    kv, ps, d, n = 2, 64, 128, 70000
+    need = -(-n // ps)
+    total = (1 << 31) // (kv * ps * d) + need + 5
+    k = torch.empty(total, kv, ps, d, dtype=F16, device=DEV)
+    v = torch.empty_like(k)
+    k[-need - 1:].normal_(generator=torch.Generator(DEV).manual_seed(1))
+    v[-need - 1:].normal_(generator=torch.Generator(DEV).manual_seed(2))
+    table = torch.arange(total - need, total, device=DEV).int().flip(0).contiguous()[None]
+    c = paged.PagedCache(k, v, table)
+    q = torch.randn(1, 8, d, device=DEV).to(F16)
+    scores = torch.zeros(1, kv, c.max_slots, device=DEV)
+    out = c.attention(q, ints([n]), scores=scores)
+    rows = lambda x: x[table[0].long()].transpose(0, 1).flatten(1, 2)[:, :n].double()
+    w = torch.softmax(q[0].double().view(kv, 4, d) @ rows(k).transpose(1, 2) / math.sqrt(d), -1)
+    want = (w @ rows(v)).view(1, 8, d)
+    near = (w @ rows(v).abs()).view(1, 8, d)
+    # the bound of oracle.paged.attend with 70000 slots in 4 chains, plus the two 16-bit half steps
+    tol = near * (half_step(F16) + (n / 4 + 200) * po.U) + want.abs() * half_step(F16) + 2.0 ** -24
+    assert ((out.double() - want).abs() <= tol).all()
+    assert torch.allclose(scores[0, :, :n].double(), w.sum(1), rtol=(n / 4 + 200) * po.U, atol=0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_captured_step_replays_with_new_lengths(dtype):
+    """Append and attention captured once; lengths, slots and pages change between replays, and two
+    graphs replayed on two streams at once do not disturb each other."""
+    kv, d, ps, heads = 2, 64, 16, 4
+    states = []
+    for seed in (1, 2):
+        k, v, table, _ = make_pool([90, 90], kv, ps, d, dtype, seed)
+        c = paged.PagedCache(k, v, table)
+        s = {"c": c, "q": torch.randn(2, heads, d, device=DEV).to(dtype), "k": torch.randn(2, kv, d, device=DEV).to(dtype),
+             "v": torch.randn(2, kv, d, device=DEV).to(dtype), "len": ints([40, 7]), "slot": ints([39, 6]), "seq": ints([0, 1]),
+             "stream": torch.cuda.Stream(), "graph": torch.cuda.CUDAGraph()}
+
+        def step(s=s):
+            qo = s["c"].append(s["q"], s["k"], s["v"], s["seq"], s["slot"])
+            return s["c"].attention(qo, s["len"])
+
+        s["step"] = step
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s["stream"]):
+            step()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(s["graph"], stream=s["stream"]):
+            s["out"] = step()
+        states.append(s)
+    for lengths in ([41, 8], [90, 1], [64, 0]):
+        for s in states:
+            s["len"].copy_(ints(lengths))
+            s["slot"].copy_(ints([max(n - 1, 0) for n in lengths]))
+            s["seq"].copy_(ints([i if n else -1 for i, n in enumerate(lengths)]))
+            s["q"].normal_()
+            s["k"].normal_()
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for s in states:
+                with torch.cuda.stream(s["stream"]):
+                    s["graph"].replay()
+        torch.cuda.synchronize()
+        for s in states:
+            got = s["out"].clone()
+            assert torch.equal(got[0], s["step"]()[0])
+            live = [i for i, n in enumerate(lengths) if n]
+            check_attention(got[live], None, rest_rows(s["c"], 0, len(live)), s["q"][live], [lengths[i] for i in live], 0, None)
+
+
+# ---- evict ------------------------------------------------------------------------------------
+
+EVICTIONS = [
+    # dtype, kv, d, page, lengths, keep, recent
+    (F32, 8, 128, 16, [257], 128, 32),
+    (BF16, 2, 128, 32, [300, 0, 40, 99, 100, 101, 1], 100, 10),
+    (F16, 1, 72, 1, [33, 5], 7, 7),
+    (F16, 3, 40, 8, [64, 65], 64, 0),
+    (F32, 2, 12, 4, [50, 50], 1, 0),
+    (F32, 2, 12, 4, [50, 50], 1, 1),
+    (BF16, 2, 256, 128, [1000, 2500], 700, 100),
+    (F16, 2, 8, 2, [4000], 3999, 1),
+]
+
+
+def run_evict(dtype, kv, d, ps, lengths, keep, recent, scores=None, seed=4):
+    k, v, table, new = make_pool(lengths, kv, ps, d, dtype, seed, fresh=-(-keep // ps) + 1, width=-(-max(lengths) // ps) + 1)
+    c = paged.PagedCache(k, v, table)
+    if scores is None:
+        g = torch.Generator(DEV).manual_seed(seed)
+        scores = (torch.rand(len(lengths), kv, c.max_slots, device=DEV, generator=g) * 20).round() / 4  # many equal
+    before = k.clone(), v.clone()
+    kept, new_len, new_sc = c.evict(ints(lengths), scores, keep, recent, new)
+    assert new_len.tolist() == [min(n, keep) for n in lengths]
+    want = before
+    for b, n in enumerate(lengths):
+        m = min(n, keep)
+        for h in range(kv):
+            idx = po.keep_slots(scores[b, h].tolist(), n, keep, recent)
+            assert kept[b, h].tolist() == idx + [-1] * (keep - m)
+            i = torch.tensor(idx, dtype=torch.long, device=DEV)
+            assert torch.equal(new_sc[b, h, :m].nan_to_num(77), scores[b, h, i].nan_to_num(77)) and not new_sc[b, h, m:].any()
+            j = torch.arange(m, device=DEV)
+            src, dst = table[b].long()[i // ps], new[b].long()[j // ps]
+            for was, pages in zip(want, (k, v)):
+                assert torch.equal(pages[dst, h, j % ps], was[src, h, i % ps])
+                was[dst, h, j % ps] = pages[dst, h, j % ps]
+    for was, pages in zip(want, (k, v)):  # nothing else is written
+        assert torch.equal(was.nan_to_num(9), pages.nan_to_num(9))
+    return c, new, new_len, new_sc
+
+
+@pytest.mark.parametrize("case", EVICTIONS, ids=str)
+def test_evict(case):
+    run_evict(*case)
+
+
+def test_evict_orders_every_kind_of_score():
+    vals = [0.0, -0.0, 1.0, math.inf, -math.inf, math.nan, 1e-45, -1e-45, 3e38, -3e38, 1.0, math.nan, -math.inf, math.inf]
+    for keep, recent in ((1, 0), (2, 0), (3, 1), (5, 0), (7, 0), (9, 2), (12, 0), (13, 0)):
+        n = len(vals)
+        sc = torch.tensor(vals, device=DEV)
+        sc = torch.cat([sc, torch.full((2 * 8 - n,), 5e30, device=DEV)])  # behind the length: must not count
+        scores = torch.zeros(1, 2, 24, device=DEV)
+        scores[0, 0, :16], scores[0, 1, :16] = sc, torch.cat([sc[:n].flip(0), sc[n:]])
+        run_evict(F32, 2, 8, 8, [n], keep, recent, scores)
+
+
+@pytest.mark.parametrize("value", [0.0, -1.5, math.nan, math.inf])
+def test_evict_equal_scores_keep_the_first(value):
+    run_evict(F16, 1, 8, 4, [3000], 1100, 50, torch.full((1, 1, 3004), value, device=DEV))
+
+
+def test_evict_long_sequence():
+    n, keep, recent = 100003, 9001, 128
+    k = torch.arange(n + 13, device=DEV, dtype=F32)[:, None].expand(-1, 4).reshape(-1, 1, 16, 4).contiguous()
+    pool = torch.cat([k, torch.zeros(600, 1, 16, 4, device=DEV)])
+    table = torch.arange(k.shape[0], device=DEV).int()[None]
+    new = torch.arange(k.shape[0], k.shape[0] + 563, device=DEV).int()[None].contiguous()
+    c = paged.PagedCache(pool, -pool, table)
+    scores = torch.rand(1, 1, c.max_slots, device=DEV).half().float()  # ties at every value
+    kept, length, sc = c.evict(ints([n]), scores, keep, recent, new)
+    idx = po.keep_slots(scores[0, 0].tolist(), n, keep, recent)
+    assert kept[0, 0].tolist() == idx and length.tolist() == [keep]
+    moved = pool[new[0].long()].reshape(-1, 4)[:keep, 0]
+    assert moved.tolist() == [float(i) for i in idx]
+    assert torch.equal(sc[0, 0, :keep], scores[0, 0, kept[0, 0].long()])
+
+
+def test_evict_flags_bad_lengths_and_pages():
+    k, v, table, new = make_pool([20, 20, 20], 1, 4, 64, F16, 8, fresh=3)
+    c = paged.PagedCache(k, v, table)
+    scores = torch.rand(1, device=DEV).expand(3, 1, c.max_slots).contiguous()
+    kept, length, _ = c.evict(ints([-2, 20, c.max_slots + 1]), scores, 10, 2, new)
+    assert device_status() == BAD and length.tolist() == [0, 10, 0]
+    assert (kept[0] == -1).all() and (kept[2] == -1).all()
+    new[1, 0] = c.num_pages
+    before = k.clone()
+    c.evict(ints([0, 20, 0]), scores, 10, 2, new)
+    assert device_status() == BAD
+    same = [p for p in range(c.num_pages) if p not in new[1].tolist()]
+    assert torch.equal(before[same].nan_to_num(9), k[same].nan_to_num(9))
+
+
+def test_python_side_refuses():
+    c = simple_cache(BF16)
+    q = torch.zeros(2, 4, 64, device=DEV, dtype=BF16)
+    k = torch.zeros(2, 2, 64, device=DEV, dtype=BF16)
+    n, i = ints([5, 3]), ints([0, 1])
+    bad = [
+        lambda: c.attention(q.float(), n), lambda: c.attention(q[:, :3], n), lambda: c.attention(q, n.long()),
+        lambda: c.attention(q, n[:1]), lambda: c.attention(q, n.cpu()), lambda: c.attention(torch.cat([q, q]), ints([1] * 4)),
+        lambda: c.attention(q, n, new_scores=torch.zeros(2, 2, c.max_slots, device=DEV)),
+        lambda: c.attention(q, n, scores=torch.zeros(2, 2, c.max_slots + 1, device=DEV)),
+        lambda: c.attention(q, n, out=torch.zeros(2, 4, 64, device=DEV)), lambda: c.attention(q[..., :32], n),
+        lambda: c.append(q, k, k[:1], i, i), lambda: c.append(q[:1], k, k, i, i), lambda: c.append(q, k, k, i, i[:1]),
+        lambda: c.append(None, k, k, i, i, out=q), lambda: c.append(q, k[:, :1], k, i, i),
+        lambda: c.append(q, k, k, i, i, i, paged.Rotary(torch.zeros(4, 33, device=DEV), torch.zeros(4, 33, device=DEV))),
+        lambda: c.append(q, k, k, i, i, None, paged.Rotary(torch.zeros(4, 32, device=DEV), torch.zeros(4, 32, device=DEV))),
+        lambda: c.append(q, k, k, i, i, i, paged.Rotary(*torch.zeros(2, 4, 32, device=DEV), q_weight=torch.ones(63, device=DEV))),
+        lambda: paged.Rotary(*torch.zeros(2, 4, 32, device=DEV), sections=(16, 8)),
+        lambda: c.evict(n, torch.zeros(2, 2, c.max_slots, device=DEV), 5, 6, ints([[0], [1]])),
+        lambda: c.evict(n, torch.zeros(2, 2, c.max_slots, device=DEV), 5, 1, ints([[0], [1]])),
+        lambda: paged.PagedCache(c.k_pages, c.v_pages[:1], c.page_table),
+        lambda: paged.PagedCache(c.k_pages, c.v_pages, c.page_table.long()),
+    ]
+    for f in bad:
+        with pytest.raises(ArgumentError):
+            f()
+    with pytest.raises(_lib.Tq4Error, match="overlaps"):
+        c.append(q, k, k, i, i, out=q)
+
+
+# ---- together, as they are used ---------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_served_batch_prompts_steps_and_eviction(dtype):
+    """Prompts appended at once, then decode steps of a ragged batch that accumulate attention
+    weights, an eviction in between, and steps over the trimmed cache: every step's output against the
+    oracle over the rows that the cache should hold."""
+    heads, kv, d, ps, pairs = 4, 2, 64, 8, 32
+    g = torch.Generator(DEV).manual_seed(3)
+    rand = lambda *s: torch.randn(*s, device=DEV, generator=g).to(dtype)
+    prompts = [21, 1, 33]
+    width = 8
+    pool_k, pool_v = (torch.full((64, kv, ps, d), math.nan, device=DEV, dtype=dtype) for _ in range(2))
+    table = torch.randperm(64, generator=torch.Generator().manual_seed(1)).int().to(DEV)[:3 * width].view(3, width).contiguous()
+    free = torch.tensor(sorted(set(range(64)) - set(table.flatten().tolist())), dtype=torch.int32, device=DEV)
+    ang = torch.arange(80, dtype=torch.float64)[:, None] * (1e4 ** (-torch.arange(pairs, dtype=torch.float64) / pairs))[None]
+    rot = paged.Rotary(ang.cos().float().to(DEV), ang.sin().float().to(DEV), sections=(8, 12, 12),
+                       q_weight=torch.rand(d, device=DEV) + 0.5, k_weight=torch.rand(d, device=DEV) + 0.5)
+    c = paged.PagedCache(pool_k, pool_v, table)
+    seq = [s for s, n in enumerate(prompts) for _ in range(n)]
+    slot = [j for n in prompts for j in range(n)]
+    t = len(seq)
+    c.append(None, rand(t, kv, d), rand(t, kv, d), ints(seq), ints(slot), ints([slot, slot, slot]), rot)
+    lengths, position = list(prompts), list(prompts)
+    scores = torch.zeros(3, kv, c.max_slots, device=DEV)
+    for step in range(8):
+        if step == 4:
+            keep, recent = 12, 4
+            new = free[:3 * 2].view(3, 2).contiguous()
+            order = [[po.keep_slots(scores[b, h].tolist(), lengths[b], keep, recent) for h in range(kv)] for b in range(3)]
+            rows = lambda pages, b, h: torch.stack([pages[table[b, j // ps], h, j % ps] for j in order[b][h]])
+            want = [[(rows(pool_k, b, h).clone(), rows(pool_v, b, h).clone()) for h in range(kv)] for b in range(3)]
+            kept, new_len, new_sc = c.evict(ints(lengths), scores, keep, recent, new)
+            lengths = new_len.tolist()
+            # the sequences go on over the new pages, with room for more
+            table = torch.cat([new, free[6:12].view(3, 2)], 1).contiguous()
+            c = paged.PagedCache(pool_k, pool_v, table)
+            scores = torch.zeros(3, kv, c.max_slots, device=DEV)
+            scores[:, :, :new_sc.shape[2]] = new_sc
+            for b in range(3):
+                for h in range(kv):
+                    for j in range(lengths[b]):
+                        assert torch.equal(pool_k[table[b, j // ps], h, j % ps], want[b][h][0][j])
+                        assert torch.equal(pool_v[table[b, j // ps], h, j % ps], want[b][h][1][j])
+        qkv = rand(3, (heads + 2 * kv) * d)
+        q, k, v = (x.unflatten(1, (-1, d)) for x in qkv.split([heads * d, kv * d, kv * d], 1))
+        p = ints([position] * 3)
+        qo = c.append(q, k, v, ints([0, 1, 2]), ints(lengths), p, rot)
+        lengths = [n + 1 for n in lengths]
+        position = [n + 1 for n in position]
+        old = scores.clone()
+        out = c.attention(qo, ints(lengths), scores=scores)
+        check_attention(out, scores, c, qo, lengths, 0, old)
+        # each sequence's weights of a step add up to one a query head
+        assert torch.allclose((scores - old).sum(-1), torch.full((3, kv), float(heads // kv), device=DEV), atol=1e-4)

@@ -30,6 +30,9 @@ EXPORTS = [
     # include/tq4_decoder.h
     "tq4_add_rmsnorm", "tq4_qk_norm_rope", "tq4_attention_decode", "tq4_attention_decode_rope",
     "tq4_matmul_fused", "tq4_silu_mul", "tq4_argmax_advance",
+    # include/tq4_paged.h
+    "tq4_paged_create", "tq4_paged_destroy", "tq4_paged_append", "tq4_paged_attention_workspace",
+    "tq4_paged_attention", "tq4_paged_evict",
 ]
 
 
@@ -47,6 +50,24 @@ class Source(ctypes.Structure):
     _fields_ = [
         ("data", ctypes.c_void_p), ("path", ctypes.c_char_p), ("offset", ctypes.c_int64),
         ("length", ctypes.c_int64),
+    ]
+
+
+class PagedDesc(ctypes.Structure):
+    """``tq4_paged_desc`` (include/tq4_paged.h)."""
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32), ("num_pages", ctypes.c_int64), ("max_seqs", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+    ]
+
+
+class RotaryDesc(ctypes.Structure):
+    """``tq4_rotary``; ``pair_axis`` is host memory."""
+    _fields_ = [
+        ("cos_table", ctypes.c_void_p), ("sin_table", ctypes.c_void_p), ("max_pos", ctypes.c_int64),
+        ("pairs", ctypes.c_int32), ("axes", ctypes.c_int32), ("pair_axis", ctypes.c_void_p),
+        ("interleaved", ctypes.c_int32), ("q_w", ctypes.c_void_p), ("k_w", ctypes.c_void_p), ("eps", ctypes.c_float),
     ]
 
 
@@ -96,6 +117,12 @@ def load():
             "tq4_sharded_rows": [vp, P(i64), P(i64)],
             "tq4_sharded_matmul": [vp, vp, i64, ctypes.c_int, vp, ctypes.c_int, vp, ctypes.c_int, vp],
             "tq4_sharded_destroy": [vp],
+            "tq4_paged_create": [P(PagedDesc), vp, vp, vp, ctypes.c_int, P(vp)],
+            "tq4_paged_destroy": [vp],
+            "tq4_paged_append": [vp, vp, i64, vp, i64, vp, i64, ctypes.c_int, i64, vp, vp, vp, P(RotaryDesc), vp, vp],
+            "tq4_paged_attention_workspace": [vp, ctypes.c_int, i64, ctypes.c_int, P(i64)],
+            "tq4_paged_attention": [vp, vp, i64, ctypes.c_int, vp, i64, ctypes.c_float, i64, vp, vp, vp, vp, i64, vp],
+            "tq4_paged_evict": [vp, vp, i64, vp, i64, i64, vp, i32, vp, vp, vp, i64, vp],
         }
         for name, args in sig.items():
             fn = getattr(lib, name)

@@ -34,7 +34,7 @@ def units():
 
 def headers():
     return [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cuh")] + [
-        os.path.join(ROOT, "include", "tq4.h"), os.path.abspath(__file__)]
+        os.path.join(ROOT, "include", h) for h in ("tq4.h", "tq4_decoder.h", "tq4_paged.h")] + [os.path.abspath(__file__)]
 
 
 def stale(target, deps):

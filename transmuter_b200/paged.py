@@ -1,0 +1,241 @@
+"""The paged key-value cache of a served q4 decoder (include/tq4_paged.h): a pool of pages that holds
+the rows of many sequences, what fills it (``PagedCache.append``: per-head RMSNorm, rotary positions
+of one or several axes, the write into pages), what reads it (``attention`` of one new token of each
+sequence) and what trims it (``evict`` by accumulated attention weight).
+
+``decoder.Q4Decoder`` runs one sequence over a contiguous f32 cache; between the projections of
+``quantized.PackedWeight`` a batch of sequences runs over this one. All tensors are CUDA tensors of
+the cache's device, calls enqueue on the current torch stream and can be captured into a CUDA graph
+(lengths, slots and page tables are read on the device). Errors follow ``quantized``: wrong arguments
+raise ``ArgumentError``; what only the device can see (a length, slot or page number out of range) is
+skipped and sets the device status (``tq4_device_status``).
+"""
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .deferred import ArgumentError
+from .quantized import TORCH_TO_TQ4
+
+FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _need(ok, message):
+    if not ok:
+        raise ArgumentError(message)
+
+
+def _dense(x, name, shape, dtype, device):
+    """A contiguous tensor of exactly this shape, type and device."""
+    _need(isinstance(x, torch.Tensor) and x.dtype == dtype and x.device == device and tuple(x.shape) == tuple(shape)
+          and x.is_contiguous(), f"paged cache: {name} must be a contiguous {dtype} {tuple(shape)} on {device}, got "
+          + (f"{x.dtype} {tuple(x.shape)} on {x.device}" if isinstance(x, torch.Tensor) else type(x).__name__))
+    return x.data_ptr()
+
+
+class Rotary:
+    """The rotary embedding of ``PagedCache.append`` and the per-head RMSNorm before it.
+
+    ``cos`` and ``sin`` are f32 tables [max_pos, pairs] (``decoder.rope_tables``), ``sections`` the
+    number of pairs that follow each axis of the positions, in order (time, height, width), or
+    ``pair_axis`` each pair's axis; one axis by default. ``interleaved`` pairs values (2i, 2i + 1)
+    instead of (i, i + pairs), and heads wider than 2 * pairs keep the rest unturned. ``q_weight`` and
+    ``k_weight`` are f32 norm weights [head_dim], None for no norm.
+    """
+
+    def __init__(self, cos, sin, sections=None, pair_axis=None, interleaved=False, q_weight=None, k_weight=None,
+                 eps=1e-6):
+        _need(isinstance(cos, torch.Tensor) and cos.dim() == 2 and cos.is_cuda,
+              "Rotary: cos must be a CUDA tensor [max_pos, pairs]")
+        max_pos, pairs = cos.shape
+        self.device, self.pairs = cos.device, pairs
+        _dense(cos, "cos", (max_pos, pairs), torch.float32, self.device)
+        _dense(sin, "sin", (max_pos, pairs), torch.float32, self.device)
+        _need(sections is None or pair_axis is None, "Rotary: sections or pair_axis, not both")
+        if sections is not None:
+            _need(sum(sections) == pairs and min(sections, default=0) >= 0,
+                  f"Rotary: sections {tuple(sections)} do not add up to {pairs} pairs")
+            pair_axis = [i for i, n in enumerate(sections) for _ in range(n)]
+            self.axes = len(sections)
+        elif pair_axis is not None:
+            _need(len(pair_axis) == pairs, f"Rotary: {len(pair_axis)} axes for {pairs} pairs")
+            self.axes = max(pair_axis, default=0) + 1
+        else:
+            pair_axis, self.axes = [0] * pairs, 1
+        _need(1 <= self.axes <= 4 and min(pair_axis, default=0) >= 0, "Rotary: 1 to 4 axes")
+        for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+            if w is not None:
+                _dense(w, name, (w.numel(),), torch.float32, self.device)
+        self.widths = {w.numel() for w in (q_weight, k_weight) if w is not None}
+        self._keep = (cos, sin, q_weight, k_weight, (ctypes.c_uint8 * max(1, pairs))(*pair_axis))
+        r = _lib.RotaryDesc()
+        r.cos_table, r.sin_table, r.max_pos, r.pairs, r.axes = cos.data_ptr(), sin.data_ptr(), max_pos, pairs, self.axes
+        r.pair_axis = ctypes.addressof(self._keep[4])
+        r.interleaved, r.eps = int(bool(interleaved)), eps
+        r.q_w = q_weight.data_ptr() if q_weight is not None else None
+        r.k_w = k_weight.data_ptr() if k_weight is not None else None
+        self._desc = r
+        self._ref = ctypes.byref(r)
+
+
+class PagedCache:
+    """A pool ``k_pages`` / ``v_pages`` [num_pages, kv_heads, page_size, head_dim] (f32, f16 or bf16)
+    with the page table int32 [max_seqs, max_pages] of the sequences in it: slot j of sequence s is
+    row j % page_size of page ``page_table[s, j // page_size]``. The tensors stay the caller's, who
+    hands out pages by writing the table."""
+
+    def __init__(self, k_pages, v_pages, page_table):
+        _need(isinstance(k_pages, torch.Tensor) and k_pages.is_cuda and k_pages.dim() == 4 and k_pages.dtype in FLOATS,
+              "PagedCache: k_pages must be a CUDA tensor [num_pages, kv_heads, page_size, head_dim], f32, f16 or bf16")
+        self.device, self.dtype = k_pages.device, k_pages.dtype
+        _dense(k_pages, "k_pages", k_pages.shape, self.dtype, self.device)
+        _dense(v_pages, "v_pages", k_pages.shape, self.dtype, self.device)
+        _need(isinstance(page_table, torch.Tensor) and page_table.dim() == 2, "PagedCache: page_table must be [max_seqs, max_pages]")
+        _dense(page_table, "page_table", page_table.shape, torch.int32, self.device)
+        self.k_pages, self.v_pages, self.page_table = k_pages, v_pages, page_table
+        self.num_pages, self.kv_heads, self.page_size, self.head_dim = k_pages.shape
+        self.max_seqs, self.max_pages = page_table.shape
+        self.max_slots = self.max_pages * self.page_size
+        d = _lib.PagedDesc()
+        d.dtype, d.kv_heads, d.head_dim, d.page_size = TORCH_TO_TQ4[self.dtype], self.kv_heads, self.head_dim, self.page_size
+        d.num_pages, d.max_seqs, d.max_pages = self.num_pages, self.max_seqs, self.max_pages
+        self._lib = _lib.load()
+        self._handle = None
+        handle = ctypes.c_void_p()
+        _lib.check(self._lib.tq4_paged_create(ctypes.byref(d), k_pages.data_ptr(), v_pages.data_ptr(),
+                                              page_table.data_ptr(), self.device.index or 0, ctypes.byref(handle)))
+        self._handle = handle
+        self._workspace = {}  # (heads, batch, with scores) -> bytes
+
+    def close(self):
+        if getattr(self, "_handle", None):
+            self._lib.tq4_paged_destroy(self._handle)
+            self._handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _stream(self):
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _rows(self, x, name, heads):
+        """x [tokens, heads, head_dim] with each token's heads contiguous; copied where they are not."""
+        _need(isinstance(x, torch.Tensor) and x.dim() == 3 and x.dtype == self.dtype and x.device == self.device
+              and x.shape[2] == self.head_dim and (heads is None or x.shape[1] == heads),
+              f"paged cache: {name} must be {self.dtype} [tokens, {heads or 'heads'}, {self.head_dim}] on {self.device}")
+        s = x.stride()
+        width = x.shape[1] * self.head_dim
+        if s[2] != 1 or (x.shape[1] > 1 and s[1] != self.head_dim) or (x.shape[0] > 1 and s[0] < width):
+            x = x.contiguous()
+            s = x.stride()
+        return x, s[0] if x.shape[0] > 1 else width
+
+    def append(self, q, k, v, seq, slot, positions=None, rotary=None, out=None):
+        """Writes the keys and values of new tokens into the cache (token t is slot ``slot[t]`` of
+        sequence ``seq[t]``; seq -1 is padding and nothing of it is touched) and returns their queries,
+        both normed and turned by ``rotary`` at ``positions`` (int32 [tokens], or [axes, tokens]).
+        q [tokens, heads, head_dim], or None when only the cache is filled; k and v [tokens, kv_heads,
+        head_dim]; views of a merged projection are read in place. ``out`` may not overlap q."""
+        k, ks = self._rows(k, "k", self.kv_heads)
+        v, vs = self._rows(v, "v", self.kv_heads)
+        tokens = k.shape[0]
+        _need(v.shape[0] == tokens, f"paged cache: {v.shape[0]} values for {tokens} keys")
+        heads, qs = 0, 0
+        if q is not None:
+            q, qs = self._rows(q, "q", None)
+            heads = q.shape[1]
+            _need(q.shape[0] == tokens and heads > 0, f"paged cache: {q.shape[0]} queries for {tokens} keys")
+            if out is None:
+                out = torch.empty((tokens, heads, self.head_dim), dtype=self.dtype, device=self.device)
+            else:
+                _dense(out, "out", (tokens, heads, self.head_dim), self.dtype, self.device)
+        else:
+            _need(out is None, "paged cache: out without q")
+        seq_p = _dense(seq, "seq", (tokens,), torch.int32, self.device)
+        slot_p = _dense(slot, "slot", (tokens,), torch.int32, self.device)
+        pos_p = ref = None
+        if rotary is not None:
+            _need(rotary.device == self.device and 2 * rotary.pairs <= self.head_dim and rotary.widths <= {self.head_dim},
+                  f"paged cache: the rotary embedding does not fit heads of {self.head_dim} values on {self.device}")
+            ref = rotary._ref
+            if rotary.pairs:
+                shape = (tokens,) if rotary.axes == 1 and positions is not None and positions.dim() == 1 else (rotary.axes, tokens)
+                pos_p = _dense(positions, "positions", shape, torch.int32, self.device)
+        _lib.check(self._lib.tq4_paged_append(
+            self._handle, q.data_ptr() if q is not None else None, qs, k.data_ptr(), ks, v.data_ptr(), vs, heads, tokens,
+            seq_p, slot_p, pos_p, ref, out.data_ptr() if out is not None else None, self._stream()))
+        return out
+
+    def attention(self, q, lengths, scale=None, window=0, scores=None, new_scores=None, out=None):
+        """Attention of one new token of each sequence b < batch over its ``lengths[b]`` slots (int32
+        [batch]; the new token's own among them), or the last ``window`` of them: [batch, heads,
+        head_dim]. Length 0 gives zeros; ``scale`` is 1 / sqrt(head_dim) by default. With ``scores``
+        (f32 [batch, kv_heads, max_pages * page_size]) each slot's softmax weights, summed over the
+        query heads of a KV head, are added to them: in place, or into ``new_scores``."""
+        q, qs = self._rows(q, "q", None)
+        batch, heads = q.shape[:2]
+        _need(0 < heads and heads % self.kv_heads == 0,
+              f"paged cache: {heads} query heads are not a multiple of {self.kv_heads} KV heads")
+        _need(batch <= self.max_seqs, f"paged cache: {batch} sequences, the page table has {self.max_seqs}")
+        len_p = _dense(lengths, "lengths", (batch,), torch.int32, self.device)
+        in_p = out_p = None
+        if scores is not None:
+            shape = (batch, self.kv_heads, self.max_slots)
+            in_p = _dense(scores, "scores", shape, torch.float32, self.device)
+            out_p = in_p if new_scores is None else _dense(new_scores, "new_scores", shape, torch.float32, self.device)
+        else:
+            _need(new_scores is None, "paged cache: new_scores without scores")
+        if out is None:
+            out = torch.empty((batch, heads, self.head_dim), dtype=self.dtype, device=self.device)
+        else:
+            _dense(out, "out", (batch, heads, self.head_dim), self.dtype, self.device)
+        key = (heads, batch, scores is not None)
+        nbytes = self._workspace.get(key)
+        if nbytes is None:
+            n = ctypes.c_int64()
+            _lib.check(self._lib.tq4_paged_attention_workspace(self._handle, heads, batch, int(key[2]), ctypes.byref(n)))
+            nbytes = self._workspace[key] = n.value
+        # a workspace of its own for each call, from torch's allocator: calls on several streams and
+        # captured graphs never share one
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        _lib.check(self._lib.tq4_paged_attention(
+            self._handle, q.data_ptr(), qs, heads, len_p, batch, 1.0 / math.sqrt(self.head_dim) if scale is None else scale,
+            window, in_p, out_p, out.data_ptr(), ws.data_ptr(), nbytes, self._stream()))
+        return out
+
+    def evict(self, lengths, scores, keep, recent, new_table, new_scores=None):
+        """Trims every sequence longer than ``keep`` to ``keep`` slots a KV head: the last ``recent``
+        and, of those before, the ones with the highest scores (equal scores: the lower slot). What
+        stays moves to the pages of ``new_table`` (int32 [batch, new_max_pages], pages that no sequence
+        of the call lists). Returns (kept slots int32 [batch, kv_heads, keep], -1 behind the last;
+        new lengths int32 [batch]; the kept slots' scores). ``new_scores`` may be given, f32 [batch,
+        kv_heads, keep or more]; a new one has 0 behind the kept slots and the width of the new table's
+        slots, as ``attention`` over it wants."""
+        _need(isinstance(lengths, torch.Tensor) and lengths.dim() == 1, "paged cache: lengths must be int32 [batch]")
+        batch = lengths.shape[0]
+        _need(batch <= self.max_seqs, f"paged cache: {batch} sequences, the page table has {self.max_seqs}")
+        len_p = _dense(lengths, "lengths", (batch,), torch.int32, self.device)
+        score_p = _dense(scores, "scores", (batch, self.kv_heads, self.max_slots), torch.float32, self.device)
+        _need(isinstance(new_table, torch.Tensor) and new_table.dim() == 2, "paged cache: new_table must be int32 [batch, pages]")
+        pages = new_table.shape[1]
+        table_p = _dense(new_table, "new_table", (batch, pages), torch.int32, self.device)
+        if new_scores is None:
+            new_scores = torch.zeros((batch, self.kv_heads, max(keep, pages * self.page_size)), dtype=torch.float32, device=self.device)
+        else:
+            _need(isinstance(new_scores, torch.Tensor) and new_scores.dim() == 3 and new_scores.shape[2] >= keep,
+                  f"paged cache: new_scores must be f32 [batch, kv_heads, {keep} or more]")
+            _dense(new_scores, "new_scores", (batch, self.kv_heads, new_scores.shape[2]), torch.float32, self.device)
+        _need(0 <= recent <= keep and 0 < keep <= pages * self.page_size,
+              f"paged cache: recent {recent} of keep {keep} slots on {pages} pages of {self.page_size}")
+        kept = torch.empty((batch, self.kv_heads, keep), dtype=torch.int32, device=self.device)
+        new_lengths = torch.empty(batch, dtype=torch.int32, device=self.device)
+        _lib.check(self._lib.tq4_paged_evict(
+            self._handle, len_p, batch, score_p, keep, recent, table_p, pages, new_lengths.data_ptr(), kept.data_ptr(),
+            new_scores.data_ptr(), new_scores.shape[2], self._stream()))
+        return kept, new_lengths, new_scores
