@@ -291,10 +291,10 @@ tq4_status tq4_paged_create(const tq4_paged_desc* desc, void* k_pages, void* v_p
     return TQ4_ERR_INVALID_ARGUMENT;
   }
   if (d.kv_heads <= 0 || d.num_pages <= 0 || d.num_pages > INT32_MAX || d.max_seqs <= 0 || d.max_pages <= 0 ||
-      (int64_t)d.max_pages * d.page_size > INT32_MAX ||
+      (int64_t)d.max_pages * d.page_size > ((int64_t)1 << 30) ||
       d.num_pages > ((int64_t)1 << 32) / d.page_size / d.kv_heads) {
-    set_error("tq4_paged_create: kv_heads, num_pages, max_seqs and max_pages must be positive, page numbers and a "
-              "sequence's slots (max_pages * page_size) below 2^31, the pool's rows (num_pages * kv_heads * page_size) "
+    set_error("tq4_paged_create: kv_heads, num_pages, max_seqs and max_pages must be positive, page numbers below "
+              "2^31, a sequence's slots (max_pages * page_size) at most 2^30, the pool's rows (num_pages * kv_heads * page_size) "
               "at most 2^32");
     return TQ4_ERR_INVALID_ARGUMENT;
   }

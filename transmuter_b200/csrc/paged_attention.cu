@@ -43,7 +43,7 @@ struct AttnArgs {
   int64_t batch, window;
   int heads, group;  // query heads, those of a KV head
   int tile, tiles;   // heads of a row, and rows of a KV head
-  int unit, ctas;    // slots of a unit; CTAs the line is cut for
+  int unit, unit_log2, ctas;  // slots of a unit; CTAs the line is cut for
   int q_even;        // q's heads are 4-byte aligned
   float scale2;      // scale * log2(e): scores are kept for exp2
   const float* scores;
@@ -64,7 +64,15 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int64_t b) {
   const int64_t n = paged_length(a.cache, a.lengths, b);
   return {(int)(a.window > 0 && n > a.window ? n - a.window : 0), (int)n};
 }
-__device__ __forceinline__ int units_of(const AttnArgs& a, Span s) { return (s.hi - s.lo + a.unit - 1) / a.unit; }
+// Units start at multiples of their size, so that one lies in one page where pages are no smaller; the
+// first of a window and the last may be partly outside the span.
+__device__ __forceinline__ int units_of(const AttnArgs& a, Span s) {
+  return (int)(((unsigned)s.hi + a.unit - 1) >> a.unit_log2) - (s.lo >> a.unit_log2);
+}
+// First slot of unit u.
+__device__ __forceinline__ int unit_slot(const AttnArgs& a, Span s, int u) {
+  return ((s.lo >> a.unit_log2) + u) << a.unit_log2;
+}
 
 // CTAs that take part: each warp of them gets a unit at least, so a short line is not spread thin.
 __device__ __forceinline__ int active_ctas(const AttnArgs& a, int64_t total) {
@@ -155,6 +163,9 @@ struct Cursor {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
   const int n = take ? 16 : 0;  // what is not taken becomes zeros, and its address is not read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() {
@@ -260,9 +271,12 @@ struct MmaFold {
     }
   }
 
-  // One unit: keys at `ks`, values behind them; bit i of `valid`: slot i counts. p0 is its first slot.
-  __device__ __forceinline__ void fold(const AttnArgs& a, const char* ks, uint32_t valid, int row_bytes, int steps,
-                                       float* w, int in_row, int G, float*, const float*) {
+  // One unit: keys at `ks`, values behind them; bit i of `valid`: slot i counts.
+  // w, if not null: where the scores of slots `from` to `to` go.
+  template <bool WHOLE>
+  __device__ __forceinline__ void fold(const AttnArgs& a, const char* ks, uint32_t valid, int row_bytes_, int steps,
+                                       float* w, int from, int to, int G, float*, const float*) {
+    const int row_bytes = WHOLE ? row_chunks<T>(DT) * 16 : row_bytes_;
     const int lane = threadIdx.x & 31;
     const uint32_t kaddr = smem_u32(ks) + (lane & 15) * row_bytes + (lane >> 4) * 16;
     const uint32_t vaddr = smem_u32(ks) + (U + (lane & 7) + (lane >> 4) * 8) * row_bytes + ((lane >> 3) & 1) * 16;
@@ -276,7 +290,7 @@ struct MmaFold {
         for (int i = 0; i < 4; ++i) s[t][n][i] = s2[n][i] = 0.f;
 #pragma unroll
       for (int k = 0; k < KS; ++k)
-        if (k < steps) {
+        if (WHOLE || k < steps) {
           uint32_t kf[4];
           ldmatrix_x4(kf, kaddr + t * 16 * row_bytes + k * 32);
 #pragma unroll
@@ -289,7 +303,7 @@ struct MmaFold {
           const int slot = t * 16 + (lane >> 2) + (i >> 1) * 8;
           s[t][n][i] = (valid >> slot) & 1 ? (s[t][n][i] + s2[n][i]) * a.scale2 : -INFINITY;
           const int g = n * 8 + (lane & 3) * 2 + (i & 1);
-          if (w && slot < in_row && g < G) w[(int64_t)slot * a.group + g] = s[t][n][i];
+          if (w && slot >= from && slot < to && g < G) w[(int64_t)slot * a.group + g] = s[t][n][i];
         }
     }
     uint32_t pf[U / 16][NT][2];
@@ -336,7 +350,7 @@ struct MmaFold {
     for (int t = 0; t < U / 16; ++t)
 #pragma unroll
       for (int k = 0; k < KS; ++k)
-        if (k < steps) {
+        if (WHOLE || k < steps) {
           uint32_t vf[4];
           ldmatrix_x4_trans(vf, vaddr + t * 16 * row_bytes + k * 32);
 #pragma unroll
@@ -412,9 +426,11 @@ struct FmaFold {
       for (int j = 0; j < COLS * 4; ++j) o[j / 4][j % 4][g] = 0.f;
   }
 
-  __device__ __forceinline__ void fold(const AttnArgs& a, const char* ks, uint32_t valid, int row_bytes, int chunks,
-                                       float* w, int in_row, int G, float* ps, const float* qs) {
-    const int lane = threadIdx.x & 31, D = a.cache.head_dim;
+  template <bool WHOLE>
+  __device__ __forceinline__ void fold(const AttnArgs& a, const char* ks, uint32_t valid, int row_bytes_, int chunks_,
+                                       float* w, int from, int to, int G, float* ps, const float* qs) {
+    const int lane = threadIdx.x & 31, D = WHOLE ? DT : a.cache.head_dim;
+    const int chunks = WHOLE ? DT / 4 : chunks_, row_bytes = WHOLE ? row_chunks<float>(DT) * 16 : row_bytes_;
     const int pg = lane & (PG - 1), slice = lane / PG;
     float v[N];  // [head][4 slots]
 #pragma unroll
@@ -447,7 +463,7 @@ struct FmaFold {
       const int slot = pg * 4 + ((idx + i) & 3), g = idx >> 2;
       v[i] = (valid >> slot) & 1 ? v[i] * a.scale2 : -INFINITY;
       mx = fmaxf(mx, v[i]);
-      if (w && slot < in_row && g < G) w[(int64_t)slot * a.group + g] = v[i];
+      if (w && slot >= from && slot < to && g < G) w[(int64_t)slot * a.group + g] = v[i];
     }
 #pragma unroll
     for (int off = 16 / TILE; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
@@ -547,7 +563,10 @@ template <typename T, int DT, int TILE> constexpr int part_smem(int head_dim) {
          (sizeof(T) == 4 ? TILE * head_dim * 4 + kPartWarps * U * TILE * 4 : 0);
 }
 
-template <typename T, int DT, int TILE>
+// WHOLE: head_dim is DT and a page holds whole units. Then a unit's keys are one run of memory, as are its
+// values: one page lookup and constant offsets instead of one row address for each chunk (the loads of
+// a unit take 30 instructions a lane instead of 300).
+template <typename T, int DT, int TILE, bool WHOLE>
 __global__ void __launch_bounds__(kPartThreads, DT <= 128 ? 2 : 1)
     attention_part_kernel(const __grid_constant__ AttnArgs a) {
   using Fold = FoldOf<T, DT, TILE>;
@@ -561,7 +580,7 @@ __global__ void __launch_bounds__(kPartThreads, DT <= 128 ? 2 : 1)
   pdl_wait();
   pdl_trigger();
   const PagedView& c = a.cache;
-  const int D = c.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int D = WHOLE ? DT : c.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int chunks = D / VN, row_bytes = row_chunks<T>(D) * 16;
   const int slot_bytes = 2 * U * row_bytes;
   char* ring = dyn + warp * kStages * slot_bytes;
@@ -595,8 +614,8 @@ __global__ void __launch_bounds__(kPartThreads, DT <= 128 ? 2 : 1)
   };
   zero_tails(ring, kStages * 2 * U);
 
-  // This warp's loads: units begin + warp, + 4, ... Lane i < U looks up the page of the unit's slot
-  // i one unit ahead of its use.
+  // This warp's loads: units begin + warp, + 4, ... A unit's page is looked up one unit ahead of its
+  // use: by lane i for slot i, or for all of them.
   Cursor next = at;
   int64_t load_x = place.begin + warp;
   if (load_x < place.end) next.step(a, rows, warp);
@@ -604,36 +623,64 @@ __global__ void __launch_bounds__(kPartThreads, DT <= 128 ? 2 : 1)
   int page = -1;
   auto look_up = [&] {
     page = -1;
-    const int p = next.span.lo + next.u * U + lane;
-    if (load_x < place.end && lane < U && p < next.span.hi)
+    if (load_x >= place.end) return;
+    const int p = unit_slot(a, next.span, next.u) + (WHOLE ? 0 : lane);
+    if (WHOLE || (lane < U && p >= next.span.lo && p < next.span.hi))
       page = c.table[(int64_t)next.b * c.max_pages + (p >> c.page_log2)];
   };
   look_up();
   auto load_unit = [&](int stage) {
     if (load_x < place.end) {
-      const int p = next.span.lo + next.u * U + lane, kvh = next.r / a.tiles;
-      const bool in = lane < U && p < next.span.hi, ok = c.page_ok(page);
+      const int p0 = unit_slot(a, next.span, next.u), kvh = next.r / a.tiles;
+      const int p = p0 + lane;
+      const bool in = lane < U && p >= next.span.lo && p < next.span.hi, ok = c.page_ok(page);
       if (in && !ok) report(kDevBadArgument);
       const uint32_t mask = __ballot_sync(0xffffffffu, in && ok);
-      // the row's number in the pool: below 2^32 (checked by tq4_paged_create)
-      const uint32_t row = (((uint32_t)page * c.kv_heads + kvh) << c.page_log2) + (p & ((1 << c.page_log2) - 1));
       if (lane == 0) valid_of[warp][stage] = mask;
       const uint32_t dst = smem_u32(ring + stage * slot_bytes);
-      int i = lane / chunks, col = lane - i * chunks;
-      for (int n = 0; n < U * chunks; n += 32) {  // every lane the same number of turns
-        const int from = min(i, U - 1);
-        const uint32_t rw = __shfl_sync(0xffffffffu, row, from);
-        const bool take = (mask >> from) & 1;
-        const int64_t off = take ? (int64_t)rw * (D * (int)sizeof(T)) + col * 16 : 0;
-        if (i < U) {
-          cp_async16(dst + i * row_bytes + col * 16, static_cast<const char*>(a.k_pages) + off, take);
-          cp_async16(dst + (U + i) * row_bytes + col * 16, static_cast<const char*>(a.v_pages) + off, take);
+      // a row's number in the pool: below 2^32 (checked by tq4_paged_create)
+      const uint32_t first = ((uint32_t)page * c.kv_heads + kvh) << c.page_log2;
+      const int in_page = (1 << c.page_log2) - 1;
+      if constexpr (WHOLE) {
+        constexpr int C = DT / VN, PITCH = row_chunks<T>(DT) * 16;
+        const int64_t off = (int64_t)(first + (p0 & in_page)) * (DT * (int)sizeof(T)) + lane * 16;
+        const char* kp = static_cast<const char*>(a.k_pages) + off;
+        const char* vp = static_cast<const char*>(a.v_pages) + off;
+        const uint32_t to = dst + (lane / C) * PITCH + (lane % C) * 16;
+        if (mask == (U == 32 ? 0xffffffffu : (1u << (U & 31)) - 1)) {
+#pragma unroll
+          for (int j = 0; j < U * C / 32; ++j) {
+            const int at_row = j * 32 / C * PITCH + j * 32 % C * 16;
+            cp_async16(to + at_row, kp + j * 512);
+            cp_async16(to + U * PITCH + at_row, vp + j * 512);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < U * C / 32; ++j) {
+            const int at_row = j * 32 / C * PITCH + j * 32 % C * 16;
+            const bool take = (mask >> (lane / C + j * 32 / C)) & 1;
+            cp_async16(to + at_row, take ? kp + j * 512 : a.k_pages, take);
+            cp_async16(to + U * PITCH + at_row, take ? vp + j * 512 : a.v_pages, take);
+          }
         }
-        i += step_row;
-        col += step_col;
-        if (col >= chunks) {
-          col -= chunks;
-          ++i;
+      } else {
+        const uint32_t row = first + (p & in_page);
+        int i = lane / chunks, col = lane - i * chunks;
+        for (int n = 0; n < U * chunks; n += 32) {  // every lane the same number of turns
+          const int from = min(i, U - 1);
+          const uint32_t rw = __shfl_sync(0xffffffffu, row, from);
+          const bool take = (mask >> from) & 1;
+          const int64_t off = take ? (int64_t)rw * (D * (int)sizeof(T)) + col * 16 : 0;
+          if (i < U) {
+            cp_async16(dst + i * row_bytes + col * 16, static_cast<const char*>(a.k_pages) + off, take);
+            cp_async16(dst + (U + i) * row_bytes + col * 16, static_cast<const char*>(a.v_pages) + off, take);
+          }
+          i += step_row;
+          col += step_col;
+          if (col >= chunks) {
+            col -= chunks;
+            ++i;
+          }
         }
       }
       load_x += kPartWarps;
@@ -658,10 +705,10 @@ __global__ void __launch_bounds__(kPartThreads, DT <= 128 ? 2 : 1)
       cp_async_wait<kStages - 2>();
       __syncwarp();
       load_unit(stage == 0 ? kStages - 1 : stage - 1);
-      const int p0 = at.span.lo + (at.u + i) * U;
+      const int p0 = unit_slot(a, at.span, at.u + i);
       float* w = a.new_scores ? a.weights + (((int64_t)at.b * c.kv_heads + kvh) * c.max_slots + p0) * a.group + g0 : nullptr;
-      fold.fold(a, ring + stage * slot_bytes, valid_of[warp][stage], row_bytes,
-                sizeof(T) == 2 ? (D + 15) / 16 : chunks, w, at.span.hi - p0, G, ps, qs);
+      fold.template fold<WHOLE>(a, ring + stage * slot_bytes, valid_of[warp][stage], row_bytes,
+                                sizeof(T) == 2 ? (D + 15) / 16 : chunks, w, at.span.lo - p0, at.span.hi - p0, G, ps, qs);
       stage = stage == kStages - 1 ? 0 : stage + 1;
     }
     // join the warps' parts; each leaves its o in the stage that it folded last
@@ -806,7 +853,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_finish_kernel(const __
       // slots before the window keep theirs
       if (at.u == 0 && now != old)
         for (int p = part * kJoinThreads + tid; p < at.span.lo; p += kWeightBlocks * kJoinThreads) now[p] = old[p];
-      const int p0 = at.span.lo + at.u * a.unit, p1 = min(at.span.hi, p0 + n * a.unit);
+      const int p0 = max(at.span.lo, unit_slot(a, at.span, at.u)), p1 = min(at.span.hi, unit_slot(a, at.span, at.u + n));
       for (int t = 0; t < a.tiles; ++t) {
         const int g0 = t * a.tile, G = min(a.tile, a.group - g0);
         const int64_t x0 = seq_first + (int64_t)(at.r + t) * at.units;
@@ -876,10 +923,12 @@ tq4_status check_attention(const tq4_paged* cache, int heads, int64_t batch) {
 template <typename T, int DT, int TILE>
 tq4_status launch_part(AttnArgs& a, cudaStream_t st) {
   a.unit = FoldOf<T, DT, TILE>::U;
+  while ((1 << a.unit_log2) < a.unit) ++a.unit_log2;
   a.ctas = DT <= 128 ? kMaxCtas : kSms;
-  static std::atomic<uint64_t> set{0};  // per device, per instantiation
-  const auto kern = attention_part_kernel<T, DT, TILE>;
-  TQ4_CUDA(set_smem_limit_once(kern, part_smem<T, DT, TILE>(DT), set));
+  const bool whole = a.cache.head_dim == DT && (1 << a.cache.page_log2) >= a.unit;
+  const auto kern = whole ? attention_part_kernel<T, DT, TILE, true> : attention_part_kernel<T, DT, TILE, false>;
+  static std::atomic<uint64_t> set[2];  // per device, per instantiation
+  TQ4_CUDA(set_smem_limit_once(kern, part_smem<T, DT, TILE>(DT), set[whole]));
   TQ4_CUDA(launch_pdl(kern, dim3(a.ctas), dim3(kPartThreads), part_smem<T, DT, TILE>(a.cache.head_dim), st, a));
   return TQ4_OK;
 }
