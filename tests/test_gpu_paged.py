@@ -338,6 +338,68 @@ def test_attention_infinite_values_stay_in_their_rows(dtype):
     assert torch.equal(out[1], good[1]) and out[0].isnan().any()
 
 
+def check_attention_long(c, q, lengths, out, old=None, new=None):
+    """check_attention in float64 on the GPU, for lengths that the oracle is too slow for. The bound is the
+    oracle's: scores off by delta, sums in four chains and their joins."""
+    kv, d, ps = c.kv_heads, c.head_dim, c.page_size
+    eps = half_step(c.dtype)
+    for b, n in enumerate(lengths):
+        if n == 0:
+            assert not out[b].any()
+            continue
+        rows = lambda x: x[c.page_table[b, :-(-n // ps)].long()].transpose(0, 1).flatten(1, 2)[:, :n].double()
+        k, v, qb = rows(c.k_pages), rows(c.v_pages), q[b].double().view(kv, -1, d)
+        w = torch.softmax(qb @ k.transpose(1, 2) / math.sqrt(d), -1)
+        delta = (qb.abs() @ k.abs().transpose(1, 2) / math.sqrt(d)).amax(-1, keepdim=True) * (d + 4) * po.U
+        rel = 2 * delta + (n / 4 + 200) * po.U
+        want, near = w @ v, w @ v.abs()
+        tol = near * rel + (0 if c.dtype == F32 else near * eps) + want.abs() * eps + 2.0 ** -24
+        assert ((out[b].double().view(kv, -1, d) - want).abs() <= tol).all()
+        if new is not None:
+            target = old[b, :, :n].double() + w.sum(1)
+            assert ((new[b, :, :n].double() - target).abs() <= (w * rel).sum(1) + target * po.U * 20).all()
+
+
+@pytest.mark.parametrize("dtype,heads,kv,d,ps,most,count", [
+    (BF16, 16, 4, 128, 16, 1500, 60), (F16, 32, 2, 64, 64, 5000, 40), (F32, 8, 8, 64, 32, 900, 50),
+    (F32, 4, 4, 128, 8, 700, 64), (F32, 24, 3, 128, 16, 3000, 20), (BF16, 8, 2, 256, 16, 4000, 20),
+    (F32, 4, 2, 256, 16, 3000, 16), (F16, 28, 4, 80, 16, 2000, 40), (BF16, 20, 1, 128, 4, 9000, 40),
+    (BF16, 12, 1, 128, 128, 200000, 1),
+], ids=str)
+@pytest.mark.parametrize("room", [1, 12])
+def test_attention_many_chunks(dtype, heads, kv, d, ps, most, count, room):
+    """Lines of several chunks a CTA, with rows of every length across their borders; with a table `room` times
+    as wide as it need be, which the chunks must not follow."""
+    g = torch.Generator().manual_seed(most)
+    lengths = [int(most * (i + 1) / count) for i in torch.randperm(count, generator=g).tolist()]
+    lengths[0], lengths[-1] = (0, 1) if count > 1 else (most, most)
+    need = [-(-n // ps) for n in lengths]
+    order = torch.randperm(sum(need), generator=g).int()
+    table = torch.full((count, max(need) * room), -1, dtype=torch.int32)
+    for b, (at, n) in enumerate(zip(np.cumsum([0] + need), need)):
+        table[b, :n] = order[at:at + n]
+    gen = torch.Generator(DEV).manual_seed(3)
+    k, v = (torch.randn(sum(need), kv, ps, d, device=DEV, dtype=dtype, generator=gen) for _ in range(2))
+    c = paged.PagedCache(k, v, table.to(DEV))
+    q = torch.randn(count, heads, d, device=DEV, dtype=dtype, generator=gen)
+    old = torch.rand(count, kv, c.max_slots, device=DEV, generator=gen)
+    new = torch.zeros_like(old)
+    out = c.attention(q, ints(lengths), scores=old, new_scores=new)
+    check_attention_long(c, q, lengths, out, old, new)
+    assert torch.equal(c.attention(q, ints(lengths)), out)
+
+
+def test_attention_short_sequences_in_a_wide_table():
+    """A table for 65536 slots with a few rows in use: most of the grid has nothing to do."""
+    lengths = [3, 0, 500, 17, 1, 260]
+    k, v, table, _ = make_pool(lengths, 8, 16, 128, BF16, 3, width=4096)
+    c = paged.PagedCache(k, v, table)
+    q = torch.randn(6, 32, 128, device=DEV).to(BF16)
+    for _ in range(20):
+        out = c.attention(q, ints(lengths))
+    check_attention(out, None, c, q, lengths, 0, None)
+
+
 def test_attention_past_2_31_values():
     """Pages beyond 2^31 values from the pool's start, and a sequence beyond 2^16 slots."""
     kv, ps, d, n = 2, 64, 128, 70000
@@ -351,15 +413,9 @@ def test_attention_past_2_31_values():
     c = paged.PagedCache(k, v, table)
     q = torch.randn(1, 8, d, device=DEV).to(F16)
     scores = torch.zeros(1, kv, c.max_slots, device=DEV)
+    old = scores.clone()
     out = c.attention(q, ints([n]), scores=scores)
-    rows = lambda x: x[table[0].long()].transpose(0, 1).flatten(1, 2)[:, :n].double()
-    w = torch.softmax(q[0].double().view(kv, 4, d) @ rows(k).transpose(1, 2) / math.sqrt(d), -1)
-    want = (w @ rows(v)).view(1, 8, d)
-    near = (w @ rows(v).abs()).view(1, 8, d)
-    # the bound of oracle.paged.attend with 70000 slots in 4 chains, plus the two 16-bit half steps
-    tol = near * (half_step(F16) + (n / 4 + 200) * po.U) + want.abs() * half_step(F16) + 2.0 ** -24
-    assert ((out.double() - want).abs() <= tol).all()
-    assert torch.allclose(scores[0, :, :n].double(), w.sum(1), rtol=(n / 4 + 200) * po.U, atol=0)
+    check_attention_long(c, q, [n], out, old, scores)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

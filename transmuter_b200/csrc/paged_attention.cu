@@ -3,36 +3,54 @@
 // A cache row is read once and used by the query heads of its KV head alone, so memory bounds this:
 // 2 * head_dim values a slot and KV head. The kernels are built around keeping loads in flight.
 //
-// The work is split over the cache's length without the host knowing any length: a sequence's
-// slots are cut into units of U (8 to 32, a warp's step), all units of all (sequence, KV head, head
-// tile) rows stand in one line, and CTA c of P takes units [c * total / P, (c + 1) * total / P) of
-// it; each CTA finds its place by a prefix sum over the lengths. Its four warps take the units in
-// turn, each through a ring of kStages units of its own that cp.async fills, also across the rows'
-// borders, so that the loads never wait for the arithmetic. A warp folds its units into a running
-// maximum m, a sum l of exp2(s - m) and an unnormalised output o (online softmax); where a row ends
-// the warps' (m, l, o) are joined in shared memory. A row that lies in one CTA is finished there, the
-// parts of others go to the workspace and a second kernel joins them in CTA order, so results depend
-// on the lengths alone.
+// The work is split over the cache's length without the host knowing any length. A sequence's slots are
+// cut into units of U (8 to 32, a warp's step), and all units of all (sequence, KV head, head tile)
+// rows stand in one line. It is cut into a share for each of the P CTAs that run at once, and each share into
+// chunks: five eighths of it, then of what is left, and so on (at most kLevels, kMinChunk units at least).
+// A CTA of the grid is a chunk; one that has begun its chunk asks the hardware for the next that has not
+// begun (cluster launch control) and goes on with it, so that its loads never pause. SMs get unequal
+// shares of the memory's rate (with one equal part for each CTA, the first was done at 125 us and the
+// last at 183 us of 64 sequences of 4096 slots): the small chunks at the end even that out.
+//   part    A CTA finds its chunk by a prefix sum over the lengths. Its warps take runs of the chunk's units
+//           (pieces, one for each warp, whoever is free) without waiting for one another: each has a ring of
+//           kStages units of its own that cp.async fills, also across the borders of rows and pieces. A warp folds
+//           units into a running maximum m, a sum l of exp2(s - m) and an unnormalised output o (online
+//           softmax). A row inside one piece is finished there; of others the parts go to the workspace.
+//           (With the warps of a CTA joined in shared memory at each row's end, that end took 2.2 us, and
+//           four of them a sixth of the kernel's time for 32 sequences of up to 4096 slots.)
+//   finish  joins the parts in the line's order, so that results depend on the lengths alone and not on
+//           who took which chunk, and adds the softmax weights to the scores.
 #include "paged.cuh"
+#include "sm100.cuh"
 
 namespace tq4 {
 
-constexpr int kPartWarps = 4;
-constexpr int kPartThreads = kPartWarps * 32;
 constexpr int kStages = 3;
 constexpr int kSms = 148;  // of a B200; only a grid's size, no CTA waits for another
-constexpr int kMaxCtas = kSms * 2;
+constexpr int kLevels = 4;
+// A chunk has three units of each of four warps at least where there are chunks to take: a warp's loads and
+// page lookups run three units ahead, so they need no more than the chunk after the current one.
+constexpr int kMinChunk = 12;
 constexpr int kMaxTile = 16;  // query heads of a row at most
 constexpr float kLog2e = 1.4426950408889634f;
 
-// What a part CTA leaves for the second kernel: where its units begin, and the row that began in an
-// earlier CTA and ends in this one, if there is one.
-struct PartInfo {
-  int64_t total;                // units in the line
-  int64_t seq_first;            // first unit of sequence b
-  int32_t b, r, u0;             // sequence, row and unit of the CTA's first; b < 0: it has none
-  int32_t end_b, end_r, first;  // the row that ends here and the CTA it began in; end_b < 0: none
+// How the line is cut: into `ctas` shares of `share` units, the first `extra` of them one longer, and each share
+// into `levels` chunks, which begin at base[level] of it. (Every share holds chunks of all sizes, so that no
+// row is made of small ones alone.)
+struct Plan {
+  int64_t total;  // units
+  int64_t share;
+  int64_t base[kLevels];
+  int32_t ctas, levels, extra;
 };
+
+struct __align__(16) Chunk {
+  int32_t b, r, u, n;  // sequence, row of it, unit of the row that the chunk begins with; units. b < 0: none
+  int32_t units;       // of that row
+  int32_t index;       // the chunk's number along the line
+  int64_t seq_first;   // the line's place where sequence b begins
+};
+__device__ __forceinline__ Chunk no_chunk() { return {-1, 0, 0, 0, 0, 0, 0}; }
 
 struct AttnArgs {
   PagedView cache;
@@ -43,16 +61,24 @@ struct AttnArgs {
   int64_t batch, window;
   int heads, group;  // query heads, those of a KV head
   int tile, tiles;   // heads of a row, and rows of a KV head
-  int unit, unit_log2, ctas;  // slots of a unit; CTAs the line is cut for
+  int unit, unit_log2;  // slots of a unit
+  int warps, ctas, levels;  // of a CTA; CTAs the line is cut for; sizes of chunks at most
   int q_even;        // q's heads are 4-byte aligned
   float scale2;      // scale * log2(e): scores are kept for exp2
   const float* scores;
   float* new_scores;
   // workspace
-  PartInfo* info;  // [kMaxCtas]
-  float* stats;    // [batch][heads][2]: m, 1 / l of rows that lie in one CTA
-  float* ml;       // [kMaxCtas][2][kMaxTile][2]: m, l of the parts of others
-  float* parts;    // [kMaxCtas][2][tile][head_dim]: their o
+  Plan* plan;
+  int64_t* seq_first;  // [batch]: the line's place where a sequence begins
+  uint8_t* ends;       // [grid * warps], by piece: 1 where a row ends that began in an earlier one
+  int4* joins;         // [grid * warps]: that row: sequence, row, the piece it began in
+  float* stats;    // [batch][heads][2]: m, 1 / l of rows that lie in one piece
+  // The parts of other rows: a piece has two at most, of a row that began in an earlier one (0) and of one that
+  // ends in a later one (1). A row's parts of a head lie in a run, so that the join streams them (with a
+  // piece's heads in a run instead, the strides met few memory channels: 26 us for 8 rows of 592 parts).
+  int pieces;      // grid * warps
+  float* ml;       // [2][tile][pieces][2]: m, l
+  float* parts;    // [2][tile][pieces][head_dim]: o
   float* weights;  // [batch][kv_heads][max_slots][group]: scores times scale2
 };
 
@@ -74,26 +100,47 @@ __device__ __forceinline__ int unit_slot(const AttnArgs& a, Span s, int u) {
   return ((s.lo >> a.unit_log2) + u) << a.unit_log2;
 }
 
-// CTAs that take part: each warp of them gets a unit at least, so a short line is not spread thin.
-__device__ __forceinline__ int active_ctas(const AttnArgs& a, int64_t total) {
-  return (int)min((int64_t)a.ctas, (total + kPartWarps - 1) / kPartWarps);
+// a / b of values that hardly ever pass 32 bits, where a division takes a fifth of the time.
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
 }
-__device__ __forceinline__ int64_t first_unit(int64_t total, int ctas, int cta) { return total * cta / ctas; }
-// The CTA whose range holds unit x.
-__device__ __forceinline__ int cta_of(int64_t total, int ctas, int64_t x) {
-  return (int)(((x + 1) * ctas - 1) / total);
+// First unit of the chunk that is number c along the line.
+__device__ __forceinline__ int64_t chunk_first(const Plan& p, int c) {
+  const int i = c / p.levels, level = c - i * p.levels;
+  return i * p.share + min(i, p.extra) + (i < p.ctas ? p.base[level] : 0);
+}
+// The chunk that holds unit x.
+__device__ __forceinline__ int chunk_of(const Plan& p, int64_t x) {
+  const int64_t longer = p.extra * (p.share + 1);
+  const int i = x < longer ? (int)divide(x, p.share + 1) : p.extra + (int)divide(x - longer, p.share);
+  const int64_t off = x - (i * p.share + min(i, p.extra));
+  int level = 0;
+  while (level + 1 < p.levels && off >= p.base[level + 1]) ++level;
+  return i * p.levels + level;
 }
 
-// The line's length, and of unit first_unit(blockIdx.x): its sequence and that sequence's first
-// unit. Each thread sums a run of sequences; the run that holds the unit is walked.
-struct Place {
-  int64_t total, begin, end, seq_first;
-  int b;
+// A chunk of n units is cut into a piece for each warp.
+__device__ __forceinline__ int piece_first(int n, int warps, int warp) { return (int)((int64_t)n * warp / warps); }
+// The piece that holds unit x, counted over all chunks.
+__device__ __forceinline__ int piece_of(const Plan& p, int warps, int64_t x) {
+  const int c = chunk_of(p, x);
+  const int64_t first = chunk_first(p, c);
+  return c * warps + (int)divide((x - first + 1) * warps - 1, chunk_first(p, c + 1) - first);
+}
+
+// The line as a CTA of THREADS threads sees it: each thread sums a run of sequences.
+template <int THREADS> struct Line {
+  Plan plan;
+  int64_t ends[THREADS];  // where each run ends
+  int per;                // sequences of a run
 };
-__device__ __forceinline__ Place find_place(const AttnArgs& a, int64_t* red) {
+// Every thread of the block calls it; ends with a barrier.
+template <int THREADS>
+__device__ __forceinline__ void make_line(const AttnArgs& a, Line<THREADS>& line, int64_t* red) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t rows = (int64_t)a.cache.kv_heads * a.tiles;
-  const int per = (int)((a.batch + kPartThreads - 1) / kPartThreads);
+  const int per = (int)((a.batch + THREADS - 1) / THREADS);
   const int b0 = (int)min((int64_t)per * tid, a.batch), b1 = (int)min((int64_t)b0 + per, a.batch);
   int64_t mine = 0;
   for (int b = b0; b < b1; ++b) mine += units_of(a, span_of(a, b)) * rows;
@@ -104,49 +151,94 @@ __device__ __forceinline__ Place find_place(const AttnArgs& a, int64_t* red) {
   }
   if (lane == 31) red[warp] = incl;
   __syncthreads();
-  Place p;
-  p.total = 0;
-  int64_t at = incl - mine;
-  for (int w = 0; w < kPartWarps; ++w) {
-    if (w == warp) at += p.total;
-    p.total += red[w];
+  int64_t before = 0, total = 0;
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w == warp) before = total;
+    total += red[w];
   }
-  const int ctas = active_ctas(a, p.total);
-  p.begin = p.end = 0;
-  p.seq_first = 0;
-  p.b = -1;
-  if ((int)blockIdx.x >= ctas) return p;  // the same for every thread
-  p.begin = first_unit(p.total, ctas, blockIdx.x);
-  p.end = first_unit(p.total, ctas, blockIdx.x + 1);
-  __syncthreads();
-  if (p.begin >= at && p.begin < at + mine) {
-    int b = b0;
-    for (;; ++b) {
-      const int64_t u = units_of(a, span_of(a, b)) * rows;
-      if (p.begin < at + u) break;
-      at += u;
+  line.ends[tid] = before + incl;
+  if (tid == 0) {
+    Plan& p = line.plan;
+    line.per = per;
+    p.total = total;
+    // a short line is not spread thin: each warp gets a unit at least
+    p.ctas = (int)min((int64_t)a.ctas, divide(total + a.warps - 1, a.warps));
+    p.levels = 0;
+    if (total > 0) {
+      p.share = divide(total, p.ctas);
+      p.extra = (int32_t)(total - p.share * p.ctas);
+      p.base[0] = 0;
+      p.levels = 1;
+      for (int64_t left = p.share; p.levels < a.levels && left >= 2 * kMinChunk; ++p.levels) {
+        left = max(left * 3 / 8, (int64_t)kMinChunk);
+        p.base[p.levels] = p.share - left;
+      }
     }
-    red[0] = b;
-    red[1] = at;
   }
   __syncthreads();
-  p.b = (int)red[0];
-  p.seq_first = red[1];
-  return p;
 }
 
+// Chunk `number` of those that the grid's CTAs are, the first of all shares and then the second, by a warp.
+template <int THREADS>
+__device__ __forceinline__ Chunk find_chunk(const AttnArgs& a, const Line<THREADS>& line, int number) {
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = (int64_t)a.cache.kv_heads * a.tiles;
+  const int level = number / line.plan.ctas, c = (number - level * line.plan.ctas) * line.plan.levels + level;
+  const int64_t x = chunk_first(line.plan, c);
+  int below = 0;  // runs that end at or before x
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; ++i) below += __popc(__ballot_sync(0xffffffffu, line.ends[i * 32 + lane] <= x));
+  Chunk k;
+  k.seq_first = below ? line.ends[below - 1] : 0;
+  for (k.b = line.per * below;; ++k.b) {
+    k.units = units_of(a, span_of(a, k.b));
+    if (x < k.seq_first + k.units * rows) break;
+    k.seq_first += k.units * rows;
+  }
+  k.r = (int)divide(x - k.seq_first, k.units);
+  k.u = (int)((x - k.seq_first) - (int64_t)k.r * k.units);
+  k.n = (int)(chunk_first(line.plan, c + 1) - x);
+  k.index = c;
+  return k;
+}
+
+// Cluster launch control: asks for a CTA of this grid that has not begun, which then never does; the
+// answer (16 bytes) arrives at `to`, completing on `bar`.
+__device__ __forceinline__ void ask_for_cta(uint32_t to, uint32_t bar) {
+  mbar_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+               ::"r"(to), "r"(bar)
+               : "memory");
+}
+// The CTA's number, or -1 where all have begun (then there is no use in asking again, and no leave).
+__device__ __forceinline__ int asked_cta(uint32_t from) {
+  uint32_t got, x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=r"(got), "=r"(x)
+      : "r"(from)
+      : "memory");
+  return got ? (int)x : -1;
+}
+
+// ---- part -----------------------------------------------------------------------------------------
 // A place in the line, stepped forward.
 struct Cursor {
   int b, r, u, units;
   Span span;
-  __device__ __forceinline__ void set(const AttnArgs& a, int b_, int64_t off) {
-    b = b_;
+  __device__ __forceinline__ void set(const AttnArgs& a, const Chunk& c) {
+    b = c.b;
+    r = c.r;
+    u = c.u;
     span = span_of(a, b);
     units = units_of(a, span);
-    r = (int)(off / units);
-    u = (int)(off - (int64_t)r * units);
   }
-  // `n` units on; the caller knows that the line goes that far.
+  // `n` units on; the caller knows that the chunk goes that far.
   __device__ __forceinline__ void step(const AttnArgs& a, int rows, int n) {
     u += n;
     while (u >= units) {
@@ -240,7 +332,7 @@ struct MmaFold {
   float o[NT][KS][4];
   float m[NT][2], l[NT][2];  // heads 2 * (lane % 4) + {0, 1} of each block
 
-  __device__ __forceinline__ void begin(const AttnArgs& a, int64_t b, int h0, int G, float*, int) {
+  __device__ __forceinline__ void load_q(const AttnArgs& a, int64_t b, int h0, int G, float*) {
     const int lane = threadIdx.x & 31, D = a.cache.head_dim;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -262,6 +354,11 @@ struct MmaFold {
           }
           qf[n][k][i] = v;
         }
+    }
+  }
+  __device__ __forceinline__ void begin() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
       m[n][0] = m[n][1] = -INFINITY;
       l[n][0] = l[n][1] = 0.f;
 #pragma unroll
@@ -302,9 +399,22 @@ struct MmaFold {
         for (int i = 0; i < 4; ++i) {
           const int slot = t * 16 + (lane >> 2) + (i >> 1) * 8;
           s[t][n][i] = (valid >> slot) & 1 ? (s[t][n][i] + s2[n][i]) * a.scale2 : -INFINITY;
-          const int g = n * 8 + (lane & 3) * 2 + (i & 1);
-          if (w && slot >= from && slot < to && g < G) w[(int64_t)slot * a.group + g] = s[t][n][i];
         }
+      if (w)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int slot = t * 16 + (lane >> 2) + h * 8, g = n * 8 + (lane & 3) * 2;
+            if (slot < from || slot >= to || g >= G) continue;
+            float* p = w + slot * a.group + g;
+            if ((a.group & 1) == 0) {
+              *reinterpret_cast<float2*>(p) = make_float2(s[t][n][2 * h], s[t][n][2 * h + 1]);
+            } else {
+              p[0] = s[t][n][2 * h];
+              if (g + 1 < G) p[1] = s[t][n][2 * h + 1];
+            }
+          }
     }
     uint32_t pf[U / 16][NT][2];
 #pragma unroll
@@ -358,8 +468,9 @@ struct MmaFold {
         }
   }
 
-  // o to os[TILE][D], m and l to ml[TILE][2].
-  __device__ __forceinline__ void end(float* os, float* ml, int D) {
+  // The row's end: of G heads, o / l to out[G][D] and m, 1 / l to ml[G][2], or where the row is not whole (out is
+  // null) o to part[G][pieces][D] and m, l to ml[G][pieces][2].
+  __device__ __forceinline__ void end(T* out, float* part, float* ml, int64_t pieces, int G, int D) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -367,15 +478,22 @@ struct MmaFold {
       for (int j = 0; j < 2; ++j) {
         for (int off = 4; off < 32; off <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], off);
         const int g = n * 8 + (lane & 3) * 2 + j;
-        if (lane < 4) {
-          ml[2 * g] = m[n][j];
-          ml[2 * g + 1] = l[n][j];
-        }
+        if (g >= G) continue;
+        const float inv = l[n][j] == 0.f ? 0.f : 1.f / l[n][j];
+        if (lane < 4)
+          *reinterpret_cast<float2*>(ml + 2 * (out ? g : g * pieces)) =
+              out ? make_float2(m[n][j] == -INFINITY ? 0.f : m[n][j], inv) : make_float2(m[n][j], l[n][j]);
+        float* to = part + g * pieces * D;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           const int d = k * 16 + (lane >> 2);
-          if (d < D) os[g * D + d] = o[n][k][j];
-          if (d + 8 < D) os[g * D + d + 8] = o[n][k][j + 2];
+          if (out) {
+            if (d < D) out[g * D + d] = from_f32<T>(o[n][k][j] * inv);
+            if (d + 8 < D) out[g * D + d + 8] = from_f32<T>(o[n][k][j + 2] * inv);
+          } else {
+            if (d < D) to[d] = o[n][k][j];
+            if (d + 8 < D) to[d + 8] = o[n][k][j + 2];
+          }
         }
       }
     }
@@ -403,13 +521,16 @@ struct FmaFold {
   float m, l;  // of the head that this lane's sums belong to
   int idx;     // they are numbers idx, idx + 1, ...: head idx / 4, slots idx % 4
 
-  __device__ __forceinline__ void begin(const AttnArgs& a, int64_t b, int h0, int G, float* qs, int) {
-    const int lane = threadIdx.x & 31, D = a.cache.head_dim;
-    for (int i = threadIdx.x; i < TILE * D; i += kPartThreads) {
-      const int g = i / D;
-      qs[i] = g < G ? static_cast<const float*>(a.q)[b * a.q_stride + (int64_t)h0 * D + i] : 0.f;
-    }
-    __syncthreads();
+  // q to the warp's qs[TILE][D]
+  __device__ __forceinline__ void load_q(const AttnArgs& a, int64_t b, int h0, int G, float* qs) {
+    const int D = a.cache.head_dim;
+    const float* src = static_cast<const float*>(a.q) + b * a.q_stride + (int64_t)h0 * D;
+    __syncwarp();
+    for (int i = threadIdx.x & 31; i < TILE * D; i += 32) qs[i] = i < G * D ? src[i] : 0.f;
+    __syncwarp();
+  }
+  __device__ __forceinline__ void begin() {
+    const int lane = threadIdx.x & 31;
     m = -INFINITY;
     l = 0.f;
     idx = 0;
@@ -535,348 +656,533 @@ struct FmaFold {
     }
   }
 
-  __device__ __forceinline__ void end(float* os, float* ml, int D) {
+  __device__ __forceinline__ void end(float* out, float* part, float* ml, int64_t pieces, int G, int D) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int off = 16 / TILE; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-    if ((lane & (32 / TILE - 1)) == 0) {
-      ml[2 * (idx >> 2)] = m;
-      ml[2 * (idx >> 2) + 1] = l * (1.f / COPIES);
+    l *= 1.f / COPIES;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if ((lane & (32 / TILE - 1)) == 0 && (idx >> 2) < G)
+      *reinterpret_cast<float2*>(ml + 2 * (idx >> 2) * (out ? 1 : pieces)) =
+          out ? make_float2(m == -INFINITY ? 0.f : m, inv) : make_float2(m, l);
+#pragma unroll
+    for (int g = 0; g < TILE; ++g) {
+      const float f = out ? __shfl_sync(0xffffffffu, inv, g * (32 / TILE)) : 1.f;
+#pragma unroll
+      for (int j = 0; j < COLS; ++j)
+        if (g < G && (lane + j * 32) * 4 < D) {
+          float* p = (out ? out + g * D : part + g * pieces * D) + (lane + j * 32) * 4;  // out may be aligned to 4 bytes only
+          p[0] = o[j][0][g] * f;
+          p[1] = o[j][1][g] * f;
+          p[2] = o[j][2][g] * f;
+          p[3] = o[j][3][g] * f;
+        }
     }
-#pragma unroll
-    for (int j = 0; j < COLS; ++j)
-      if ((lane + j * 32) * 4 < D)
-#pragma unroll
-        for (int g = 0; g < TILE; ++g)
-          *reinterpret_cast<float4*>(os + g * D + (lane + j * 32) * 4) =
-              make_float4(o[j][0][g], o[j][1][g], o[j][2][g], o[j][3][g]);
   }
 };
 
 template <typename T, int DT, int TILE>
 using FoldOf = std::conditional_t<sizeof(T) == 4, FmaFold<DT, TILE>, MmaFold<T, DT, TILE>>;
 
-// Dynamic shared memory: the rings, then for f32 the queries and each warp's weights.
+// Warps of a CTA: four, or three where f32 queries of 8 heads need their room.
+template <typename T, int TILE> constexpr int kWarpsOf = sizeof(T) == 4 && TILE == 8 ? 3 : 4;
+
+// Dynamic shared memory: the rings, then for f32 each warp's queries and softmax weights.
 template <typename T, int DT, int TILE> constexpr int part_smem(int head_dim) {
   constexpr int U = FoldOf<T, DT, TILE>::U;
-  return kPartWarps * kStages * 2 * U * row_chunks<T>(head_dim) * 16 +
-         (sizeof(T) == 4 ? TILE * head_dim * 4 + kPartWarps * U * TILE * 4 : 0);
+  return kWarpsOf<T, TILE> * (kStages * 2 * U * row_chunks<T>(head_dim) * 16 +
+                              (sizeof(T) == 4 ? TILE * head_dim * 4 + U * TILE * 4 : 0));
 }
 
 // WHOLE: head_dim is DT and a page holds whole units. Then a unit's keys are one run of memory, as are its
 // values: one page lookup and constant offsets instead of one row address for each chunk (the loads of
 // a unit take 30 instructions a lane instead of 300).
 template <typename T, int DT, int TILE, bool WHOLE>
-__global__ void __launch_bounds__(kPartThreads, DT <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(kWarpsOf<T, TILE> * 32, DT <= 128 ? 2 : 1)
     attention_part_kernel(const __grid_constant__ AttnArgs a) {
   using Fold = FoldOf<T, DT, TILE>;
-  constexpr int U = Fold::U;
+  constexpr int U = Fold::U, WARPS = kWarpsOf<T, TILE>, THREADS = WARPS * 32;
   constexpr int VN = 16 / sizeof(T);
-  __shared__ int64_t red[2 * kPartWarps];
-  __shared__ float ml[kPartWarps][TILE][2];
-  __shared__ uint32_t valid_of[kPartWarps][kStages];
-  __shared__ int free_of[kPartWarps];
+  __shared__ uint32_t valid_of[WARPS][kStages];
+  __shared__ Line<THREADS> line;
+  __shared__ int64_t red[WARPS];
+  __shared__ Chunk chunk_at[4];  // the CTA's chunks after the first, by turns
+  __shared__ __align__(16) uint4 answer;
+  __shared__ __align__(8) uint64_t known[4];  // chunk_at[i] holds a chunk
+  __shared__ __align__(8) uint64_t taken[4];  // all its pieces have been taken
+  __shared__ __align__(8) uint64_t answered;
+  __shared__ int s_abort, s_taken, s_ask, s_answers;
   extern __shared__ __align__(16) char dyn[];
-  pdl_wait();
-  pdl_trigger();
   const PagedView& c = a.cache;
   const int D = WHOLE ? DT : c.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int chunks = D / VN, row_bytes = row_chunks<T>(D) * 16;
   const int slot_bytes = 2 * U * row_bytes;
   char* ring = dyn + warp * kStages * slot_bytes;
-  float* qs = reinterpret_cast<float*>(dyn + kPartWarps * kStages * slot_bytes);
-  float* ps = qs + TILE * D + warp * U * TILE;
+  float* qs = reinterpret_cast<float*>(dyn + WARPS * kStages * slot_bytes) + warp * TILE * (D + U);
+  float* ps = qs + TILE * D;
   const int rows = c.kv_heads * a.tiles;
 
-  // sequences without slots give zeros
-  for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x)
-    if (span_of(a, b).hi == 0)
-      for (int i = tid; i < a.heads * D; i += kPartThreads) static_cast<T*>(a.out)[b * a.heads * D + i] = from_f32<T>(0.f);
-
-  const Place place = find_place(a, red);
-  PartInfo info = {place.total, place.seq_first, -1, 0, 0, -1, 0, 0};
-  if (place.b < 0) {
-    if (tid == 0) a.info[blockIdx.x] = info;
-    return;
+  // 16-bit rows of an odd number of 16-byte chunks: their last 16-value step reads one more, kept at zero
+  if (sizeof(T) == 2 && (chunks & 1))
+    for (int i = lane; i < kStages * 2 * U; i += 32)
+      *reinterpret_cast<uint4*>(ring + i * row_bytes + chunks * 16) = make_uint4(0, 0, 0, 0);
+  if (tid == 0) {
+    s_abort = 0;
+    s_taken = WARPS;  // each warp has a piece of the first chunk
+    s_ask = (int)gridDim.x > a.ctas;
+    s_answers = 0;
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(smem_u32(&known[i]), 1);
+      mbar_init(smem_u32(&taken[i]), WARPS);
+    }
+    mbar_init(smem_u32(&answered), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async_smem();
   }
-  const int ctas = active_ctas(a, place.total);
-  Cursor at;  // the row being folded
-  at.set(a, place.b, place.begin - place.seq_first);
-  info.b = at.b;
-  info.r = at.r;
-  info.u0 = at.u;
-
-  // 16-bit rows of an odd number of chunks: their last 16-value step reads one more, kept at zero
-  auto zero_tails = [&](char* rows_at, int n) {
-    if (sizeof(T) == 2 && (chunks & 1))
-      for (int i = lane; i < n; i += 32)
-        *reinterpret_cast<uint4*>(rows_at + i * row_bytes + chunks * 16) = make_uint4(0, 0, 0, 0);
-  };
-  zero_tails(ring, kStages * 2 * U);
-
-  // This warp's loads: units begin + warp, + 4, ... A unit's page is looked up one unit ahead of its
-  // use: by lane i for slot i, or for all of them.
-  Cursor next = at;
-  int64_t load_x = place.begin + warp;
-  if (load_x < place.end) next.step(a, rows, warp);
-  const int step_row = 32 / chunks, step_col = 32 % chunks;  // from a lane's chunk to its next
-  int page = -1;
-  auto look_up = [&] {
-    page = -1;
-    if (load_x >= place.end) return;
-    const int p = unit_slot(a, next.span, next.u) + (WHOLE ? 0 : lane);
-    if (WHOLE || (lane < U && p >= next.span.lo && p < next.span.hi))
-      page = c.table[(int64_t)next.b * c.max_pages + (p >> c.page_log2)];
-  };
-  look_up();
-  auto load_unit = [&](int stage) {
-    if (load_x < place.end) {
-      const int p0 = unit_slot(a, next.span, next.u), kvh = next.r / a.tiles;
-      const int p = p0 + lane;
-      const bool in = lane < U && p >= next.span.lo && p < next.span.hi, ok = c.page_ok(page);
-      if (in && !ok) report(kDevBadArgument);
-      const uint32_t mask = __ballot_sync(0xffffffffu, in && ok);
-      if (lane == 0) valid_of[warp][stage] = mask;
-      const uint32_t dst = smem_u32(ring + stage * slot_bytes);
-      // a row's number in the pool: below 2^32 (checked by tq4_paged_create)
-      const uint32_t first = ((uint32_t)page * c.kv_heads + kvh) << c.page_log2;
-      const int in_page = (1 << c.page_log2) - 1;
-      if constexpr (WHOLE) {
-        constexpr int C = DT / VN, PITCH = row_chunks<T>(DT) * 16;
-        const int64_t off = (int64_t)(first + (p0 & in_page)) * (DT * (int)sizeof(T)) + lane * 16;
-        const char* kp = static_cast<const char*>(a.k_pages) + off;
-        const char* vp = static_cast<const char*>(a.v_pages) + off;
-        const uint32_t to = dst + (lane / C) * PITCH + (lane % C) * 16;
-        if (mask == (U == 32 ? 0xffffffffu : (1u << (U & 31)) - 1)) {
-#pragma unroll
-          for (int j = 0; j < U * C / 32; ++j) {
-            const int at_row = j * 32 / C * PITCH + j * 32 % C * 16;
-            cp_async16(to + at_row, kp + j * 512);
-            cp_async16(to + U * PITCH + at_row, vp + j * 512);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < U * C / 32; ++j) {
-            const int at_row = j * 32 / C * PITCH + j * 32 % C * 16;
-            const bool take = (mask >> (lane / C + j * 32 / C)) & 1;
-            cp_async16(to + at_row, take ? kp + j * 512 : a.k_pages, take);
-            cp_async16(to + U * PITCH + at_row, take ? vp + j * 512 : a.v_pages, take);
-          }
-        }
-      } else {
-        const uint32_t row = first + (p & in_page);
-        int i = lane / chunks, col = lane - i * chunks;
-        for (int n = 0; n < U * chunks; n += 32) {  // every lane the same number of turns
-          const int from = min(i, U - 1);
-          const uint32_t rw = __shfl_sync(0xffffffffu, row, from);
-          const bool take = (mask >> from) & 1;
-          const int64_t off = take ? (int64_t)rw * (D * (int)sizeof(T)) + col * 16 : 0;
-          if (i < U) {
-            cp_async16(dst + i * row_bytes + col * 16, static_cast<const char*>(a.k_pages) + off, take);
-            cp_async16(dst + (U + i) * row_bytes + col * 16, static_cast<const char*>(a.v_pages) + off, take);
-          }
-          i += step_row;
-          col += step_col;
-          if (col >= chunks) {
-            col -= chunks;
-            ++i;
-          }
-        }
-      }
-      load_x += kPartWarps;
-      if (load_x < place.end) next.step(a, rows, kPartWarps);
-      look_up();
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) load_unit(s);
-
-  Fold fold;
-  int stage = 0;  // of the next unit to fold; the one before it is free
-  for (int64_t x = place.begin; x < place.end;) {
-    const int n = (int)min(place.end - x, (int64_t)(at.units - at.u));
-    const int kvh = at.r / a.tiles, g0 = (at.r - kvh * a.tiles) * TILE;
-    const int G = min(TILE, a.group - g0), h0 = kvh * a.group + g0;
-    fold.begin(a, at.b, h0, G, qs, 0);
-    // this warp's units of the row: those at a distance of warp, modulo kPartWarps, from the first
-    const int mine = (int)((warp - (x - place.begin)) & (kPartWarps - 1));
-    for (int i = mine; i < n; i += kPartWarps) {
-      cp_async_wait<kStages - 2>();
-      __syncwarp();
-      load_unit(stage == 0 ? kStages - 1 : stage - 1);
-      const int p0 = unit_slot(a, at.span, at.u + i);
-      float* w = a.new_scores ? a.weights + (((int64_t)at.b * c.kv_heads + kvh) * c.max_slots + p0) * a.group + g0 : nullptr;
-      fold.template fold<WHOLE>(a, ring + stage * slot_bytes, valid_of[warp][stage], row_bytes,
-                                sizeof(T) == 2 ? (D + 15) / 16 : chunks, w, at.span.lo - p0, at.span.hi - p0, G, ps, qs);
-      stage = stage == kStages - 1 ? 0 : stage + 1;
-    }
-    // join the warps' parts; each leaves its o in the stage that it folded last
-    const int free_stage = stage == 0 ? kStages - 1 : stage - 1;
-    __syncwarp();
-    fold.end(reinterpret_cast<float*>(ring + free_stage * slot_bytes), &ml[warp][0][0], D);
-    if (lane == 0) free_of[warp] = free_stage;
-    __syncthreads();
-    const bool whole = n == at.units;
-    const int64_t slot = (int64_t)blockIdx.x * 2 + (at.u > 0 ? 0 : 1);  // at most two rows of a CTA are not whole
-    for (int i = tid; i < G * D; i += kPartThreads) {
-      const int g = i / D;
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kPartWarps; ++w) M = fmaxf(M, ml[w][g][0]);
-      const float f = M == -INFINITY ? 0.f : M;
-      float num = 0.f, den = 0.f;
-#pragma unroll
-      for (int w = 0; w < kPartWarps; ++w) {
-        const float e = ex2(ml[w][g][0] - f);
-        num = fmaf(e, reinterpret_cast<const float*>(dyn + (w * kStages + free_of[w]) * slot_bytes)[i], num);
-        den = fmaf(e, ml[w][g][1], den);
-      }
-      if (whole) {
-        static_cast<T*>(a.out)[((int64_t)at.b * a.heads + h0) * D + i] = from_f32<T>(den == 0.f ? 0.f : num / den);
-        if (i == g * D) {
-          a.stats[((int64_t)at.b * a.heads + h0 + g) * 2] = f;
-          a.stats[((int64_t)at.b * a.heads + h0 + g) * 2 + 1] = den == 0.f ? 0.f : 1.f / den;
-        }
-      } else {
-        a.parts[slot * TILE * D + i] = num;
-        if (i == g * D) {
-          a.ml[(slot * kMaxTile + g) * 2] = M;
-          a.ml[(slot * kMaxTile + g) * 2 + 1] = den;
-        }
-      }
-    }
-    if (!whole && at.u > 0 && at.u + n == at.units) {
-      info.end_b = at.b;
-      info.end_r = at.r;
-      info.first = cta_of(place.total, ctas, x - at.u);
-    }
-    __syncthreads();
-    zero_tails(ring + free_stage * slot_bytes, 2 * U);
-    x += n;
-    if (x < place.end) at.step(a, rows, n);
-  }
-  if (tid == 0) a.info[blockIdx.x] = info;
-}
-
-// ---- the second kernel --------------------------------------------------------------------------
-// Part slot of CTA k for a row that began in CTA `first`.
-__device__ __forceinline__ int64_t part_slot(int k, int first) { return (int64_t)k * 2 + (k == first); }
-
-// m (0 where nothing counts) and 1 / l of head g of a row that lies in CTAs first to last.
-__device__ __forceinline__ float2 part_stats(const AttnArgs& a, int first, int last, int g) {
-  float M = -INFINITY, den = 0.f;
-  for (int k = first; k <= last; ++k) M = fmaxf(M, a.ml[(part_slot(k, first) * kMaxTile + g) * 2]);
-  const float f = M == -INFINITY ? 0.f : M;
-  for (int k = first; k <= last; ++k) {
-    const float* p = a.ml + (part_slot(k, first) * kMaxTile + g) * 2;
-    den = fmaf(ex2(p[0] - f), p[1], den);
-  }
-  return make_float2(f, den == 0.f ? 0.f : 1.f / den);
-}
-
-constexpr int kJoinThreads = 256;
-constexpr int kJoinCols = 32;                         // 4-value columns of a block
-constexpr int kJoinParts = kJoinThreads / kJoinCols;  // parts added at once
-constexpr int kWeightBlocks = 4;                      // blocks that share a CTA's units
-
-// blockIdx.x: a part CTA. blockIdx.y below join_blocks: some columns of the row that ends in it are
-// joined; above: the weights of its units are added to the scores.
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) attention_finish_kernel(const __grid_constant__ AttnArgs a, int join_blocks) {
+  __syncthreads();
   pdl_wait();
   pdl_trigger();
-  __shared__ float4 sums[kJoinParts][kJoinCols];
-  __shared__ float2 st[kMaxTile];
-  const PagedView& c = a.cache;
-  const int D = c.head_dim, tid = threadIdx.x;
-  const PartInfo info = a.info[blockIdx.x];
-  if ((int)blockIdx.y < join_blocks) {
-    if (info.end_b < 0) return;
-    const int kvh = info.end_r / a.tiles, g0 = (info.end_r - kvh * a.tiles) * a.tile;
-    const int G = min(a.tile, a.group - g0), h0 = kvh * a.group + g0;
-    const int first = info.first, last = blockIdx.x;
-    const int col = blockIdx.y * kJoinCols + tid % kJoinCols, j = tid / kJoinCols;
-    const int g = col * 4 / D;  // D is a multiple of 4
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    float2 ms = make_float2(0.f, 0.f);
-    if (g < G) {
-      ms = part_stats(a, first, last, g);
-#pragma unroll 4
-      for (int k = first + j; k <= last; k += kJoinParts) {
-        const int64_t slot = part_slot(k, first);
-        const float e = ex2(a.ml[(slot * kMaxTile + g) * 2] - ms.x);
-        const float4 v = *reinterpret_cast<const float4*>(a.parts + slot * a.tile * D + col * 4);
-        s.x = fmaf(e, v.x, s.x);
-        s.y = fmaf(e, v.y, s.y);
-        s.z = fmaf(e, v.z, s.z);
-        s.w = fmaf(e, v.w, s.w);
-      }
+  make_line(a, line, red);
+  const int n_chunks = line.plan.ctas * line.plan.levels;
+  if (blockIdx.x == 0) {
+    if (tid == 0) *a.plan = line.plan;
+    int64_t at = tid ? line.ends[tid - 1] : 0;
+    for (int b = tid * line.per; b < (tid + 1) * line.per && b < a.batch; ++b) {
+      a.seq_first[b] = at;
+      at += (int64_t)units_of(a, span_of(a, b)) * rows;
     }
-    sums[j][tid % kJoinCols] = s;
-    __syncthreads();
-    if (j == 0 && g < G) {
-      for (int i = 1; i < kJoinParts; ++i) {
-        const float4 v = sums[i][tid];
-        s.x += v.x;
-        s.y += v.y;
-        s.z += v.z;
-        s.w += v.w;
-      }
-      T* out = static_cast<T*>(a.out) + ((int64_t)info.end_b * a.heads + h0) * D + col * 4;
-      out[0] = from_f32<T>(s.x * ms.y);
-      out[1] = from_f32<T>(s.y * ms.y);
-      out[2] = from_f32<T>(s.z * ms.y);
-      out[3] = from_f32<T>(s.w * ms.y);
-    }
-    return;
   }
-  // scores: the rows of the heads' first tile, each with the heads of all tiles
-  if (info.b < 0) return;
-  const int ctas = active_ctas(a, info.total), rows = c.kv_heads * a.tiles;
-  const int64_t end = first_unit(info.total, ctas, blockIdx.x + 1);
-  int64_t x = first_unit(info.total, ctas, blockIdx.x), seq_first = info.seq_first;
-  Cursor at;
-  at.b = info.b;
-  at.span = span_of(a, at.b);
-  at.units = units_of(a, at.span);
-  at.r = info.r;
-  at.u = info.u0;
-  const int part = blockIdx.y - join_blocks;
-  while (x < end) {
-    const int n = (int)min(end - x, (int64_t)(at.units - at.u));
-    const int kvh = at.r / a.tiles;
-    if (at.r == kvh * a.tiles) {
-      const int64_t row = (int64_t)at.b * c.kv_heads + kvh;
-      const float* old = a.scores + row * c.max_slots;
-      float* now = a.new_scores + row * c.max_slots;
-      // slots before the window keep theirs
-      if (at.u == 0 && now != old)
-        for (int p = part * kJoinThreads + tid; p < at.span.lo; p += kWeightBlocks * kJoinThreads) now[p] = old[p];
-      const int p0 = max(at.span.lo, unit_slot(a, at.span, at.u)), p1 = min(at.span.hi, unit_slot(a, at.span, at.u + n));
-      for (int t = 0; t < a.tiles; ++t) {
-        const int g0 = t * a.tile, G = min(a.tile, a.group - g0);
-        const int64_t x0 = seq_first + (int64_t)(at.r + t) * at.units;
-        const int first = cta_of(info.total, ctas, x0), last = cta_of(info.total, ctas, x0 + at.units - 1);
-        __syncthreads();
-        if (tid < G) {
-          const float* s = a.stats + ((int64_t)at.b * a.heads + kvh * a.group + g0 + tid) * 2;
-          st[tid] = first == last ? make_float2(s[0], s[1]) : part_stats(a, first, last, tid);
+  if ((int)blockIdx.x >= n_chunks) return;  // the grid was made for longer sequences
+
+  // ---- the CTA's pieces ----
+  // Piece j is one of chunk j / WARPS of the CTA (0 is blockIdx.x). Warps take them by ticket; who takes the
+  // first of a chunk makes it known to the others and asks for the one after it. That happens in the chunks'
+  // order: a warp waits with one piece at most. Numbers beyond the line's chunks are asked for too, so that
+  // they need not be launched.
+  const bool seamless = line.plan.levels > 1;  // loads go on into the next piece; a single level's may be too short
+  auto draw = [&] {
+    if (lane == 0 && s_ask) ask_for_cta(smem_u32(&answer), smem_u32(&answered));
+    __syncwarp();
+  };
+  auto drawn = [&]() -> Chunk {
+    while (s_ask) {
+      const int n = s_answers;
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&answered), n & 1, &s_abort, kDevTimeoutAttn))) break;
+      const int got = asked_cta(smem_u32(&answer));
+      fence_proxy_async_smem();  // the answer is read before the next one is written
+      __syncwarp();
+      if (lane == 0) {
+        s_answers = n + 1;
+        if (got < 0) s_ask = 0;
+      }
+      __syncwarp();
+      if (got >= n_chunks) draw();
+      else if (got >= 0) return find_chunk(a, line, got);
+    }
+    return no_chunk();
+  };
+  struct Piece {
+    Chunk k;
+    int w;  // which of the chunk's
+  };
+  auto take = [&]() -> Piece {
+    int j = 0;
+    if (lane == 0) j = atomicAdd(&s_taken, 1);
+    j = __shfl_sync(0xffffffffu, j, 0);
+    const int s = j / WARPS, at = s & 3, phase = (s - 1) >> 2;
+    Piece p = {no_chunk(), j - s * WARPS};
+    if (p.w == 0) {
+      const Chunk k = drawn();
+      if (s > 4 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&taken[at]), (phase - 1) & 1, &s_abort, kDevTimeoutAttn))) return p;
+      if (lane == 0) {
+        chunk_at[at] = k;
+        mbar_arrive(smem_u32(&known[at]));
+      }
+      __syncwarp();
+      if (k.b >= 0) draw();
+    }
+    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&known[at]), phase & 1, &s_abort, kDevTimeoutAttn))) return p;
+    p.k = chunk_at[at];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&taken[at]));
+    return p;
+  };
+
+  // ---- this warp's loads ----
+  // A unit's page is looked up one unit ahead of its use: by lane i for slot i, or for all of them.
+  Piece cur = {find_chunk(a, line, blockIdx.x), warp};  // being folded
+  Piece coming = cur;                                   // being loaded
+  if (warp == 0) draw();
+  Cursor next;
+  int load_left;
+  auto enter = [&] {  // sets the loads to `coming`
+    load_left = 0;
+    if (coming.k.b < 0) return;
+    const int first = piece_first(coming.k.n, WARPS, coming.w);
+    load_left = piece_first(coming.k.n, WARPS, coming.w + 1) - first;
+    if (load_left == 0) return;
+    next.set(a, coming.k);
+    if (first) next.step(a, rows, first);
+  };
+  auto advance = [&] {
+    if (--load_left > 0) {
+      next.step(a, rows, 1);
+    } else if (seamless) {
+      coming = take();
+      enter();
+    }
+  };
+  auto look_up = [&]() -> int {
+    if (load_left == 0) return -1;
+    const int p = unit_slot(a, next.span, next.u) + (WHOLE ? 0 : lane);
+    if (WHOLE || (lane < U && p >= next.span.lo && p < next.span.hi))
+      return c.table[(int64_t)next.b * c.max_pages + (p >> c.page_log2)];
+    return -1;
+  };
+  auto load_unit = [&](int stage, const Cursor& next, int page) {
+    const int p0 = unit_slot(a, next.span, next.u), kvh = next.r / a.tiles;
+    const int p = p0 + lane;
+    const bool in = lane < U && p >= next.span.lo && p < next.span.hi, ok = c.page_ok(page);
+    if (in && !ok) report(kDevBadArgument);
+    const uint32_t mask = __ballot_sync(0xffffffffu, in && ok);
+    if (lane == 0) valid_of[warp][stage] = mask;
+    const uint32_t dst = smem_u32(ring + stage * slot_bytes);
+    // a row's number in the pool: below 2^32 (checked by tq4_paged_create)
+    const uint32_t first = ((uint32_t)page * c.kv_heads + kvh) << c.page_log2;
+    const int in_page = (1 << c.page_log2) - 1;
+    if constexpr (WHOLE) {
+      constexpr int C = DT / VN, PITCH = row_chunks<T>(DT) * 16;
+      const int64_t off = (int64_t)(first + (p0 & in_page)) * (DT * (int)sizeof(T)) + lane * 16;
+      const char* kp = static_cast<const char*>(a.k_pages) + off;
+      const char* vp = static_cast<const char*>(a.v_pages) + off;
+      const uint32_t to = dst + (lane / C) * PITCH + (lane % C) * 16;
+      if (mask == (U == 32 ? 0xffffffffu : (1u << (U & 31)) - 1)) {
+#pragma unroll
+        for (int j = 0; j < U * C / 32; ++j) {
+          const int at_row = j * 32 / C * PITCH + j * 32 % C * 16;
+          cp_async16(to + at_row, kp + j * 512);
+          cp_async16(to + U * PITCH + at_row, vp + j * 512);
         }
-        __syncthreads();
-        for (int p = p0 + part * kJoinThreads + tid; p < p1; p += kWeightBlocks * kJoinThreads) {
-          const float* w = a.weights + (row * c.max_slots + p) * a.group + g0;
-          float sum = 0.f;
-          for (int g = 0; g < G; ++g) sum = fmaf(ex2(w[g] - st[g].x), st[g].y, sum);
-          now[p] = (t == 0 ? old[p] : now[p]) + sum;
+      } else {
+#pragma unroll
+        for (int j = 0; j < U * C / 32; ++j) {
+          const int at_row = j * 32 / C * PITCH + j * 32 % C * 16;
+          const bool take = (mask >> (lane / C + j * 32 / C)) & 1;
+          cp_async16(to + at_row, take ? kp + j * 512 : a.k_pages, take);
+          cp_async16(to + U * PITCH + at_row, take ? vp + j * 512 : a.v_pages, take);
+        }
+      }
+    } else {
+      const int step_row = 32 / chunks, step_col = 32 % chunks;  // from a lane's chunk to its next
+      const uint32_t row = first + (p & in_page);
+      int i = lane / chunks, col = lane - i * chunks;
+      for (int n = 0; n < U * chunks; n += 32) {  // every lane the same number of turns
+        const int from = min(i, U - 1);
+        const uint32_t rw = __shfl_sync(0xffffffffu, row, from);
+        const bool take = (mask >> from) & 1;
+        const int64_t off = take ? (int64_t)rw * (D * (int)sizeof(T)) + col * 16 : 0;
+        if (i < U) {
+          cp_async16(dst + i * row_bytes + col * 16, static_cast<const char*>(a.k_pages) + off, take);
+          cp_async16(dst + (U + i) * row_bytes + col * 16, static_cast<const char*>(a.v_pages) + off, take);
+        }
+        i += step_row;
+        col += step_col;
+        if (col >= chunks) {
+          col -= chunks;
+          ++i;
         }
       }
     }
-    x += n;
-    if (x < end) {
-      if (at.r + 1 == rows) seq_first += (int64_t)rows * at.units;
-      at.step(a, rows, n);
+  };
+
+  // ---- folding ----
+  Fold fold;
+  int stage = 0;  // of the next unit to fold; the one before it is free
+  enter();
+  int page = -1;
+  auto start = [&] {  // the first two units' pages are looked up together
+    static_assert(kStages == 3);
+    const Cursor c0 = next;
+    const bool any = load_left > 0;
+    const int page0 = look_up();
+    if (any) advance();
+    const int page1 = look_up();
+    if (any) load_unit(stage, c0, page0);
+    cp_async_commit();
+    if (load_left > 0) {
+      load_unit(stage == kStages - 1 ? 0 : stage + 1, next, page1);
+      advance();
     }
+    cp_async_commit();
+    page = look_up();
+  };
+  start();
+  for (;;) {
+    const int piece = cur.k.index * WARPS + cur.w;
+    const int first = piece_first(cur.k.n, WARPS, cur.w);
+    int left = piece_first(cur.k.n, WARPS, cur.w + 1) - first;
+    bool ends = false;
+    if (left == 0)  // parts that the second kernel passes over
+      for (int i = lane; i < 2 * TILE; i += 32) a.ml[((int64_t)i * a.pieces + piece) * 2] = -INFINITY;
+    Cursor at;
+    if (left > 0) {
+      at.set(a, cur.k);
+      if (first) at.step(a, rows, first);
+    }
+    while (left > 0) {
+      const int n = min(left, at.units - at.u);
+      const int kvh = at.r / a.tiles, g0 = (at.r - kvh * a.tiles) * TILE;
+      const int G = min(TILE, a.group - g0), h0 = kvh * a.group + g0;
+      fold.load_q(a, at.b, h0, G, qs);
+      fold.begin();
+      for (int i = 0; i < n; ++i) {
+        cp_async_wait<kStages - 2>();
+        __syncwarp();
+        if (load_left > 0) {
+          load_unit(stage == 0 ? kStages - 1 : stage - 1, next, page);
+          advance();
+          page = look_up();
+        }
+        cp_async_commit();
+        const int p0 = unit_slot(a, at.span, at.u + i);
+        float* w = a.new_scores ? a.weights + (((int64_t)at.b * c.kv_heads + kvh) * c.max_slots + p0) * a.group + g0 : nullptr;
+        fold.template fold<WHOLE>(a, ring + stage * slot_bytes, valid_of[warp][stage], row_bytes,
+                                  sizeof(T) == 2 ? (D + 15) / 16 : chunks, w, at.span.lo - p0, at.span.hi - p0, G, ps, qs);
+        stage = stage == kStages - 1 ? 0 : stage + 1;
+      }
+      if (n == at.units) {
+        const int64_t head = (int64_t)at.b * a.heads + h0;
+        fold.end(static_cast<T*>(a.out) + head * D, nullptr, a.stats + head * 2, 0, G, D);
+      } else {
+        const int64_t to = (int64_t)(at.u > 0 ? 0 : TILE) * a.pieces + piece;
+        fold.end(nullptr, a.parts + to * D, a.ml + to * 2, a.pieces, G, D);
+        if (at.u > 0 && at.u + n == at.units) {
+          ends = true;
+          // it is the piece's first row, which the piece begins with unit at.u of
+          const int64_t x = chunk_first(line.plan, cur.k.index) + first - at.u;
+          if (lane == 0) a.joins[piece] = make_int4(at.b, at.r, piece_of(line.plan, WARPS, x), 0);
+        }
+      }
+      left -= n;
+      if (left > 0) at.step(a, rows, n);
+    }
+    if (lane == 0) a.ends[piece] = ends;
+    if (!seamless) {
+      coming = take();
+      cp_async_wait<0>();
+      __syncwarp();
+      enter();
+      start();
+    }
+    cur = coming;
+    if (cur.k.b < 0 || *static_cast<volatile int*>(&s_abort)) break;
+  }
+  cp_async_wait<0>();
+  if (s_abort && s_ask) mbar_drain(smem_u32(&answered), s_answers & 1);  // an answer may still be on its way
+}
+
+// ---- finish ---------------------------------------------------------------------------------------
+constexpr int kFinishThreads = 256;
+constexpr int kFinishBlocks = kSms * 4;  // of joins, and about as many of scores
+constexpr int kMaxJoins = 2 * kSms * kLevels * 4;  // a piece ends one at most
+
+// (m, l) pairs joined; m of 0 weights is -inf.
+__device__ __forceinline__ float2 join(float2 x, float2 y) {
+  const float m = fmaxf(x.x, y.x), f = m == -INFINITY ? 0.f : m;
+  return make_float2(m, x.y * ex2(x.x - f) + y.y * ex2(y.x - f));
+}
+
+// The pieces in which a row ends that began in an earlier one, in order, to list; their number. By the block.
+__device__ __forceinline__ int list_joins(const AttnArgs& a, int pieces, uint16_t* list, int* red) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int count = 0;
+  for (int base = 0; base < pieces; base += kFinishThreads * 16) {
+    const int p0 = base + tid * 16;
+    uint32_t bits = 0;  // of 16 pieces
+    if (p0 < pieces) {
+      const uint4 f = *reinterpret_cast<const uint4*>(a.ends + p0);
+      const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (p0 + i < pieces && ((w[i / 4] >> (i % 4 * 8)) & 255) == 1) bits |= 1u << i;
+    }
+    int incl = __popc(bits);
+    for (int off = 1; off < 32; off <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += y;
+    }
+    if (lane == 31) red[warp] = incl;
+    __syncthreads();
+    int at = count + incl - __popc(bits);
+    for (int w = 0; w < kFinishThreads / 32; ++w) {
+      if (w < warp) at += red[w];
+      count += red[w];
+    }
+    for (; bits; bits &= bits - 1) list[at++] = (uint16_t)(p0 + __ffs(bits) - 1);
+    __syncthreads();
+  }
+  return count;
+}
+
+// Head g of the row that ends in piece `last`, `cols` columns of 4 values from col0, by the block: `cols`
+// threads have the columns, and groups of them every so many-th part.
+template <typename T>
+__device__ __forceinline__ void join_head(const AttnArgs& a, int last, int g, int cols, int col0, float4* sums, float2* mls) {
+  const int D = a.cache.head_dim, tid = threadIdx.x;
+  const int4 row = a.joins[last];
+  const int kvh = row.y / a.tiles, g0 = (row.y - kvh * a.tiles) * a.tile, first = row.z;
+  if (g >= a.group - g0) return;  // the same for the block
+  const int lanes = kFinishThreads / cols, j = tid / cols, col = tid - j * cols, d = (col0 + col) * 4;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  float2 ml = make_float2(-INFINITY, 0.f);
+  constexpr int kAtOnce = 4;  // parts whose loads are in flight together
+  if (d < D)
+    for (int p0 = first + j; p0 <= last; p0 += kAtOnce * lanes) {
+      float2 x[kAtOnce];
+      float4 v[kAtOnce];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int p = p0 + i * lanes;
+        const int64_t at = (int64_t)((p == first ? a.tile : 0) + g) * a.pieces + p;
+        x[i] = make_float2(-INFINITY, 0.f);
+        if (p <= last) {
+          x[i] = *reinterpret_cast<const float2*>(a.ml + at * 2);
+          v[i] = *reinterpret_cast<const float4*>(a.parts + at * D + d);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        if (x[i].x == -INFINITY) continue;  // nothing counted, or nothing written
+        const float m = fmaxf(ml.x, x[i].x), e0 = ex2(ml.x - m), e1 = ex2(x[i].x - m);
+        ml = make_float2(m, ml.y * e0 + x[i].y * e1);
+        s.x = s.x * e0 + v[i].x * e1;
+        s.y = s.y * e0 + v[i].y * e1;
+        s.z = s.z * e0 + v[i].z * e1;
+        s.w = s.w * e0 + v[i].w * e1;
+      }
+    }
+  // the groups' sums, by halves
+  int n = 1;
+  while (n < min(lanes, last - first + 1)) n *= 2;
+  __syncthreads();
+  sums[tid] = s;
+  mls[tid] = ml;
+  __syncthreads();
+  for (n /= 2; n > 0; n /= 2) {
+    if (j < n) {
+      const float2 x = mls[tid + n * cols];
+      const float4 v = sums[tid + n * cols];
+      const float m = fmaxf(ml.x, x.x), f = m == -INFINITY ? 0.f : m, e0 = ex2(ml.x - f), e1 = ex2(x.x - f);
+      ml = make_float2(m, ml.y * e0 + x.y * e1);
+      s = make_float4(s.x * e0 + v.x * e1, s.y * e0 + v.y * e1, s.z * e0 + v.z * e1, s.w * e0 + v.w * e1);
+      sums[tid] = s;
+      mls[tid] = ml;
+    }
+    __syncthreads();
+  }
+  if (j == 0 && d < D) {
+    const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
+    T* out = static_cast<T*>(a.out) + ((int64_t)row.x * a.heads + kvh * a.group + g0 + g) * D + d;
+    out[0] = from_f32<T>(s.x * inv);
+    out[1] = from_f32<T>(s.y * inv);
+    out[2] = from_f32<T>(s.z * inv);
+    out[3] = from_f32<T>(s.w * inv);
+  }
+}
+
+// The softmax weights of the slots of row (b, kvh) from `from`, every stride-th of them a thread's, added to
+// the scores. VEC: heads that one load brings.
+template <int VEC>
+__device__ __forceinline__ void add_weights(const AttnArgs& a, const Plan& plan, int64_t row, int from, int stride,
+                                            float2* st) {
+  static_assert(kFinishThreads == 16 * kMaxTile, "16 threads a head");
+  const PagedView& c = a.cache;
+  const int tid = threadIdx.x;
+  const int64_t b = row / c.kv_heads;
+  const int kvh = (int)(row - b * c.kv_heads);
+  const Span sp = span_of(a, b);
+  if (sp.hi == 0) return;
+  const int units = units_of(a, sp);
+  const float* old = a.scores + row * c.max_slots;
+  float* now = a.new_scores + row * c.max_slots;
+  if (now != old)  // slots before the window keep theirs
+    for (int p = from + tid; p < sp.lo; p += stride) now[p] = old[p];
+  for (int t = 0; t < a.tiles; ++t) {
+    const int t0 = t * a.tile, G = min(a.tile, a.group - t0);
+    const int64_t x = a.seq_first[b] + (int64_t)(kvh * a.tiles + t) * units;
+    const int first = piece_of(plan, a.warps, x), last = piece_of(plan, a.warps, x + units - 1);
+    __syncthreads();
+    if (first == last) {
+      const float* s = a.stats + (b * a.heads + kvh * a.group + t0) * 2;
+      if (tid < G) st[tid] = make_float2(s[2 * tid], s[2 * tid + 1]);
+    } else {
+      const int g = min(tid / 16, G - 1), j = tid & 15;
+      float2 ml = make_float2(-INFINITY, 0.f);
+#pragma unroll 4
+      for (int p = first + j; p <= last; p += 16) {
+        const float2 y = *reinterpret_cast<const float2*>(a.ml + ((int64_t)((p == first ? a.tile : 0) + g) * a.pieces + p) * 2);
+        if (y.x != -INFINITY) ml = join(ml, y);
+      }
+      for (int off = 8; off > 0; off >>= 1)
+        ml = join(ml, make_float2(__shfl_xor_sync(0xffffffffu, ml.x, off), __shfl_xor_sync(0xffffffffu, ml.y, off)));
+      if (j == 0 && tid / 16 < G) st[g] = make_float2(ml.x == -INFINITY ? 0.f : ml.x, ml.y == 0.f ? 0.f : 1.f / ml.y);
+    }
+    __syncthreads();
+    const float* w = a.weights + row * c.max_slots * a.group + t0;
+#pragma unroll 4
+    for (int p = sp.lo + from + tid; p < sp.hi; p += stride) {
+      float sum = 0.f;
+      for (int g = 0; g < G; g += VEC) {
+        float y[VEC];
+        const float* src = w + (int64_t)p * a.group + g;
+        if constexpr (VEC == 4) *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(src);
+        else if constexpr (VEC == 2) *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(src);
+        else y[0] = src[0];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum = fmaf(ex2(y[i] - st[g + i].x), st[g + i].y, sum);
+      }
+      now[p] = (t == 0 ? old[p] : now[p]) + sum;
+    }
+  }
+}
+
+// kFinishBlocks blocks, the even ones of the first where there are scores too: joins. The others: scores, `pieces`
+// blocks a row.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kFinishThreads, 4)
+    attention_finish_kernel(const __grid_constant__ AttnArgs a, int pieces) {
+  __shared__ float4 sums[kFinishThreads];
+  __shared__ float2 mls[kFinishThreads];
+  __shared__ Plan plan;
+  __shared__ uint16_t list[kMaxJoins];
+  __shared__ int red[kFinishThreads / 32];
+  pdl_wait();
+  pdl_trigger();
+  const int D = a.cache.head_dim, tid = threadIdx.x;
+  const int scorers = gridDim.x - kFinishBlocks, both = 2 * min(scorers, kFinishBlocks);
+  const int index = (int)blockIdx.x < both ? blockIdx.x / 2 : blockIdx.x - both / 2;
+  if ((int)blockIdx.x < both ? (blockIdx.x & 1) == 0 : scorers < kFinishBlocks) {
+    const int n = list_joins(a, a.plan->ctas * a.plan->levels * a.warps, list, red);
+    // A task is a head's columns. Few rows have many parts each: their columns are spread over more blocks,
+    // whose threads then have more groups for the parts.
+    const int G = min(a.tile, a.group), all = D / 4;
+    int cols = 2;
+    while (cols < all) cols *= 2;
+    while (cols > 8 && n * G * ((all + cols / 2 - 1) / (cols / 2)) <= kFinishBlocks) cols /= 2;
+    const int splits = (all + cols - 1) / cols, tasks = n * G * splits;
+    for (int task = index; task < tasks; task += kFinishBlocks) {
+      const int head = task / splits, row = head / G;
+      join_head<T>(a, list[row], head - row * G, cols, (task - head * splits) * cols, sums, mls);
+    }
+    // sequences without slots give zeros
+    for (int64_t b = index; b < a.batch; b += kFinishBlocks)
+      if (span_of(a, b).hi == 0)
+        for (int i = tid; i < a.heads * D; i += kFinishThreads) static_cast<T*>(a.out)[b * a.heads * D + i] = from_f32<T>(0.f);
+  } else {
+    if (tid == 0) plan = *a.plan;
+    __syncthreads();
+    const int64_t row = index / pieces;
+    add_weights<VEC>(a, plan, row, (int)(index - row * pieces) * kFinishThreads, pieces * kFinishThreads, mls);
   }
 }
 
@@ -888,17 +1194,46 @@ int head_tile(const tq4_paged_desc& d, int heads) {
   return group > 8 ? 16 : 8;
 }
 
+// How a call is cut, from what the host knows of it.
+struct Shape {
+  int tile, tiles, unit, unit_log2, warps, ctas, levels;
+  int64_t grid;  // as many chunks as sequences that fill the page table would give
+};
+Shape shape_of(const tq4_paged_desc& d, int heads, int64_t batch) {
+  Shape s;
+  const int group = heads / d.kv_heads;
+  s.tile = head_tile(d, heads);
+  s.tiles = (group + s.tile - 1) / s.tile;
+  // the folds' U and the kernels' warps and residence
+  s.unit = d.dtype == TQ4_F32 ? (d.head_dim <= 64 ? 16 : 8) : (d.head_dim <= 64 ? 32 : 16);
+  s.unit_log2 = s.unit == 8 ? 3 : s.unit == 16 ? 4 : 5;
+  s.warps = d.dtype == TQ4_F32 && s.tile == 8 ? 3 : 4;
+  s.ctas = d.head_dim <= 128 ? 2 * kSms : kSms;
+  const int64_t slots = (int64_t)d.max_pages * d.page_size;
+  const int64_t most = batch * d.kv_heads * s.tiles * ((slots + s.unit - 1) / s.unit + 1);
+  s.levels = 1;
+  for (int64_t left = most / s.ctas; s.levels < kLevels && left >= 2 * kMinChunk; ++s.levels)
+    left = std::max<int64_t>(left * 3 / 8, kMinChunk);
+  s.grid = s.levels > 1 ? (int64_t)s.ctas * s.levels : std::min<int64_t>(s.ctas, (most + s.warps - 1) / s.warps);
+  return s;
+}
+
 // Offsets of the workspace's parts, in bytes, each a multiple of 16.
 struct Workspace {
-  int64_t stats, ml, parts, weights, bytes;
+  int64_t seq_first, ends, joins, stats, ml, parts, weights, bytes;
 };
 Workspace workspace_of(const tq4_paged_desc& d, int heads, int64_t batch, bool with_scores) {
   auto up = [](int64_t n) { return (n + 15) / 16 * 16; };
+  const Shape s = shape_of(d, heads, batch);
+  const int64_t slots = s.grid * s.warps * 2 * s.tile;
   Workspace w;
-  w.stats = up(kMaxCtas * sizeof(PartInfo));
+  w.seq_first = up(sizeof(Plan));
+  w.ends = w.seq_first + up(batch * 8);
+  w.joins = w.ends + up(s.grid * s.warps);
+  w.stats = w.joins + s.grid * s.warps * 16;
   w.ml = w.stats + up(batch * heads * 2 * 4);
-  w.parts = w.ml + kMaxCtas * 2 * kMaxTile * 2 * 4;
-  w.weights = w.parts + up((int64_t)kMaxCtas * 2 * head_tile(d, heads) * d.head_dim * 4);
+  w.parts = w.ml + up(slots * 2 * 4);
+  w.weights = w.parts + up(slots * d.head_dim * 4);
   w.bytes = w.weights + (with_scores ? up(batch * heads * (int64_t)d.max_pages * d.page_size * 4) : 0);
   return w;
 }
@@ -921,42 +1256,48 @@ tq4_status check_attention(const tq4_paged* cache, int heads, int64_t batch) {
 }
 
 template <typename T, int DT, int TILE>
-tq4_status launch_part(AttnArgs& a, cudaStream_t st) {
-  a.unit = FoldOf<T, DT, TILE>::U;
-  while ((1 << a.unit_log2) < a.unit) ++a.unit_log2;
-  a.ctas = DT <= 128 ? kMaxCtas : kSms;
+tq4_status launch_part(AttnArgs& a, int64_t grid, cudaStream_t st) {
+  if (a.unit != FoldOf<T, DT, TILE>::U || a.warps != kWarpsOf<T, TILE>) {
+    set_error("tq4_paged_attention: the call was cut for other kernels");
+    return TQ4_ERR_UNSUPPORTED;
+  }
   const bool whole = a.cache.head_dim == DT && (1 << a.cache.page_log2) >= a.unit;
   const auto kern = whole ? attention_part_kernel<T, DT, TILE, true> : attention_part_kernel<T, DT, TILE, false>;
   static std::atomic<uint64_t> set[2];  // per device, per instantiation
   TQ4_CUDA(set_smem_limit_once(kern, part_smem<T, DT, TILE>(DT), set[whole]));
-  TQ4_CUDA(launch_pdl(kern, dim3(a.ctas), dim3(kPartThreads), part_smem<T, DT, TILE>(a.cache.head_dim), st, a));
+  TQ4_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(a.warps * 32), part_smem<T, DT, TILE>(a.cache.head_dim), st, a));
   return TQ4_OK;
 }
 
 template <typename T, int TILE>
-tq4_status launch_width(AttnArgs& a, cudaStream_t st) {
+tq4_status launch_width(AttnArgs& a, int64_t grid, cudaStream_t st) {
   const int D = a.cache.head_dim;
-  if (D <= 64) return launch_part<T, 64, TILE>(a, st);
-  if (D <= 128) return launch_part<T, 128, TILE>(a, st);
-  return launch_part<T, 256, TILE>(a, st);
+  if (D <= 64) return launch_part<T, 64, TILE>(a, grid, st);
+  if (D <= 128) return launch_part<T, 128, TILE>(a, grid, st);
+  return launch_part<T, 256, TILE>(a, grid, st);
 }
 
 template <typename T>
-tq4_status launch_attention(AttnArgs& a, cudaStream_t st) {
+tq4_status launch_attention(AttnArgs& a, int64_t grid, cudaStream_t st) {
   if constexpr (sizeof(T) == 4) {
     switch (a.tile) {
-      case 1: TQ4_TRY((launch_width<T, 1>(a, st))); break;
-      case 2: TQ4_TRY((launch_width<T, 2>(a, st))); break;
-      case 4: TQ4_TRY((launch_width<T, 4>(a, st))); break;
-      default: TQ4_TRY((launch_width<T, 8>(a, st))); break;
+      case 1: TQ4_TRY((launch_width<T, 1>(a, grid, st))); break;
+      case 2: TQ4_TRY((launch_width<T, 2>(a, grid, st))); break;
+      case 4: TQ4_TRY((launch_width<T, 4>(a, grid, st))); break;
+      default: TQ4_TRY((launch_width<T, 8>(a, grid, st))); break;
     }
   } else {
-    if (a.tile == 8) TQ4_TRY((launch_width<T, 8>(a, st)));
-    else TQ4_TRY((launch_width<T, 16>(a, st)));
+    if (a.tile == 8) TQ4_TRY((launch_width<T, 8>(a, grid, st)));
+    else TQ4_TRY((launch_width<T, 16>(a, grid, st)));
   }
-  const int join = (std::min(a.tile, a.group) * a.cache.head_dim / 4 + kJoinCols - 1) / kJoinCols;
-  TQ4_CUDA(launch_pdl(attention_finish_kernel<T>, dim3(a.ctas, join + (a.new_scores ? kWeightBlocks : 0)),
-                      dim3(kJoinThreads), 0, st, a, join));
+  const auto finish = a.group % 4 == 0   ? attention_finish_kernel<T, 4>
+                      : a.group % 2 == 0 ? attention_finish_kernel<T, 2>
+                                         : attention_finish_kernel<T, 1>;
+  const int64_t rows = a.batch * a.cache.kv_heads;
+  const int pieces = (int)std::min<int64_t>(std::max<int64_t>(1, 2 * kFinishBlocks / rows),
+                                            (a.cache.max_slots + kFinishThreads - 1) / kFinishThreads);
+  const int64_t blocks = kFinishBlocks + (a.new_scores ? rows * pieces : 0);
+  TQ4_CUDA(launch_pdl(finish, dim3((unsigned)blocks), dim3(kFinishThreads), 0, st, a, pieces));
   return TQ4_OK;
 }
 
@@ -1015,24 +1356,38 @@ tq4_status tq4_paged_attention(const tq4_paged* cache, const void* q, int64_t q_
   a.window = window;
   a.heads = heads;
   a.group = heads / d.kv_heads;
-  a.tile = head_tile(d, heads);
-  a.tiles = (a.group + a.tile - 1) / a.tile;
+  const Shape shape = shape_of(d, heads, batch);
+  a.tile = shape.tile;
+  a.tiles = shape.tiles;
+  a.unit = shape.unit;
+  a.unit_log2 = shape.unit_log2;
+  a.warps = shape.warps;
+  a.ctas = shape.ctas;
+  a.levels = shape.levels;
   a.q_even = (reinterpret_cast<uintptr_t>(q) & 3) == 0 && (q_stride & 1) == 0;
   a.scale2 = scale * kLog2e;
   a.scores = scores;
   a.new_scores = new_scores;
   char* w = static_cast<char*>(workspace);
-  a.info = reinterpret_cast<PartInfo*>(w);
+  a.plan = reinterpret_cast<Plan*>(w);
+  a.seq_first = reinterpret_cast<int64_t*>(w + ws.seq_first);
+  a.ends = reinterpret_cast<uint8_t*>(w + ws.ends);
+  a.joins = reinterpret_cast<int4*>(w + ws.joins);
   a.stats = reinterpret_cast<float*>(w + ws.stats);
   a.ml = reinterpret_cast<float*>(w + ws.ml);
+  a.pieces = (int)shape.grid * shape.warps;
   a.parts = reinterpret_cast<float*>(w + ws.parts);
   a.weights = reinterpret_cast<float*>(w + ws.weights);
+  if (batch * d.kv_heads * a.tiles > ((int64_t)1 << 30)) {
+    set_error("tq4_paged_attention: more than 2^30 rows of sequences and KV heads");
+    return TQ4_ERR_INVALID_ARGUMENT;
+  }
   DeviceGuard guard(cache->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (d.dtype) {
-    case TQ4_F16: return launch_attention<__half>(a, st);
-    case TQ4_BF16: return launch_attention<__nv_bfloat16>(a, st);
-    default: return launch_attention<float>(a, st);
+    case TQ4_F16: return launch_attention<__half>(a, shape.grid, st);
+    case TQ4_BF16: return launch_attention<__nv_bfloat16>(a, shape.grid, st);
+    default: return launch_attention<float>(a, shape.grid, st);
   }
 }
 
