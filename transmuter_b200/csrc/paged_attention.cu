@@ -27,7 +27,7 @@ namespace tq4 {
 
 constexpr int kStages = 3;
 constexpr int kSms = 148;  // of a B200; only a grid's size, no CTA waits for another
-constexpr int kLevels = 4;
+constexpr int kLevels = 6;
 // A chunk has three units of each of four warps at least where there are chunks to take: a warp's loads and
 // page lookups run three units ahead, so they need no more than the chunk after the current one.
 constexpr int kMinChunk = 12;
@@ -993,19 +993,25 @@ __device__ __forceinline__ float2 join(float2 x, float2 y) {
 }
 
 // The pieces in which a row ends that began in an earlier one, in order, to list; their number. By the block.
-__device__ __forceinline__ int list_joins(const AttnArgs& a, int pieces, uint16_t* list, int* red) {
+__device__ __forceinline__ int list_joins(const AttnArgs& a, uint16_t* list, int* red) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int count = 0;
-  for (int base = 0; base < pieces; base += kFinishThreads * 16) {
-    const int p0 = base + tid * 16;
-    uint32_t bits = 0;  // of 16 pieces
-    if (p0 < pieces) {
-      const uint4 f = *reinterpret_cast<const uint4*>(a.ends + p0);
-      const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+  constexpr int kRounds = (kMaxJoins + kFinishThreads * 16 - 1) / (kFinishThreads * 16);
+  uint4 f[kRounds];
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (p0 + i < pieces && ((w[i / 4] >> (i % 4 * 8)) & 255) == 1) bits |= 1u << i;
-    }
+  for (int r = 0; r < kRounds; ++r) {  // of 16 pieces a thread; those beyond the line's hold anything
+    const int p0 = (r * kFinishThreads + tid) * 16;
+    if (p0 < a.pieces) f[r] = *reinterpret_cast<const uint4*>(a.ends + p0);
+  }
+  const int pieces = a.plan->ctas * a.plan->levels * a.warps;
+  int count = 0;
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int p0 = (r * kFinishThreads + tid) * 16;
+    const uint32_t w[4] = {f[r].x, f[r].y, f[r].z, f[r].w};
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (p0 + i < pieces && ((w[i / 4] >> (i % 4 * 8)) & 255) == 1) bits |= 1u << i;
     int incl = __popc(bits);
     for (int off = 1; off < 32; off <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, incl, off);
@@ -1129,19 +1135,35 @@ __device__ __forceinline__ void add_weights(const AttnArgs& a, const Plan& plan,
     }
     __syncthreads();
     const float* w = a.weights + row * c.max_slots * a.group + t0;
-#pragma unroll 4
-    for (int p = sp.lo + from + tid; p < sp.hi; p += stride) {
-      float sum = 0.f;
-      for (int g = 0; g < G; g += VEC) {
-        float y[VEC];
-        const float* src = w + (int64_t)p * a.group + g;
-        if constexpr (VEC == 4) *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(src);
-        else if constexpr (VEC == 2) *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(src);
-        else y[0] = src[0];
+    constexpr int kAtOnce = 4;  // slots of a thread whose loads are in flight together
+    for (int p0 = sp.lo + from + tid; p0 < sp.hi; p0 += kAtOnce * stride) {
+      float was[kAtOnce], sum[kAtOnce];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sum = fmaf(ex2(y[i] - st[g + i].x), st[g + i].y, sum);
+      for (int k = 0; k < kAtOnce; ++k) {
+        const int p = p0 + k * stride;
+        was[k] = p < sp.hi ? (t == 0 ? old[p] : now[p]) : 0.f;
+        sum[k] = 0.f;
       }
-      now[p] = (t == 0 ? old[p] : now[p]) + sum;
+      for (int g = 0; g < G; g += VEC) {
+        float y[kAtOnce][VEC];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          const int p = min(p0 + k * stride, sp.hi - 1);
+          const float* src = w + (int64_t)p * a.group + g;
+          if constexpr (VEC == 4) *reinterpret_cast<float4*>(y[k]) = *reinterpret_cast<const float4*>(src);
+          else if constexpr (VEC == 2) *reinterpret_cast<float2*>(y[k]) = *reinterpret_cast<const float2*>(src);
+          else y[k][0] = src[0];
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float2 ml = st[g + i];
+#pragma unroll
+          for (int k = 0; k < kAtOnce; ++k) sum[k] = fmaf(ex2(y[k][i] - ml.x), ml.y, sum[k]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k)
+        if (p0 + k * stride < sp.hi) now[p0 + k * stride] = was[k] + sum[k];
     }
   }
 }
@@ -1162,13 +1184,13 @@ __global__ void __launch_bounds__(kFinishThreads, 4)
   const int scorers = gridDim.x - kFinishBlocks, both = 2 * min(scorers, kFinishBlocks);
   const int index = (int)blockIdx.x < both ? blockIdx.x / 2 : blockIdx.x - both / 2;
   if ((int)blockIdx.x < both ? (blockIdx.x & 1) == 0 : scorers < kFinishBlocks) {
-    const int n = list_joins(a, a.plan->ctas * a.plan->levels * a.warps, list, red);
+    const int n = list_joins(a, list, red);
     // A task is a head's columns. Few rows have many parts each: their columns are spread over more blocks,
     // whose threads then have more groups for the parts.
     const int G = min(a.tile, a.group), all = D / 4;
     int cols = 2;
     while (cols < all) cols *= 2;
-    while (cols > 8 && n * G * ((all + cols / 2 - 1) / (cols / 2)) <= kFinishBlocks) cols /= 2;
+    while (cols > 4 && n * G * ((all + cols / 2 - 1) / (cols / 2)) <= kFinishBlocks) cols /= 2;
     const int splits = (all + cols - 1) / cols, tasks = n * G * splits;
     for (int task = index; task < tasks; task += kFinishBlocks) {
       const int head = task / splits, row = head / G;

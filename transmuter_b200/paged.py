@@ -28,12 +28,19 @@ def _need(ok, message):
         raise ArgumentError(message)
 
 
-def _dense(x, name, shape, dtype, device):
-    """A contiguous tensor of exactly this shape, type and device."""
-    _need(isinstance(x, torch.Tensor) and x.dtype == dtype and x.device == device and tuple(x.shape) == tuple(shape)
-          and x.is_contiguous(), f"paged cache: {name} must be a contiguous {dtype} {tuple(shape)} on {device}, got "
-          + (f"{x.dtype} {tuple(x.shape)} on {x.device}" if isinstance(x, torch.Tensor) else type(x).__name__))
+def _pointer(x, name, shape, dtype, device):
+    """The address of a contiguous tensor of exactly this shape, type and device."""
+    # (a call makes up to nine of these checks in the time of one launch: the message is only made for a refusal)
+    if not (isinstance(x, torch.Tensor) and x.dtype is dtype and x.shape == shape and x.device == device
+            and x.is_contiguous()):
+        got = f"{x.dtype} {tuple(x.shape)} on {x.device}" if isinstance(x, torch.Tensor) else type(x).__name__
+        raise ArgumentError(f"paged cache: {name} must be a contiguous {dtype} {tuple(shape)} on {device}, got {got}")
     return x.data_ptr()
+
+
+# The stream's address without the Stream object around it (2.2 us of a call otherwise).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 class Rotary:
@@ -52,8 +59,8 @@ class Rotary:
               "Rotary: cos must be a CUDA tensor [max_pos, pairs]")
         max_pos, pairs = cos.shape
         self.device, self.pairs = cos.device, pairs
-        _dense(cos, "cos", (max_pos, pairs), torch.float32, self.device)
-        _dense(sin, "sin", (max_pos, pairs), torch.float32, self.device)
+        _pointer(cos, "cos", (max_pos, pairs), torch.float32, self.device)
+        _pointer(sin, "sin", (max_pos, pairs), torch.float32, self.device)
         _need(sections is None or pair_axis is None, "Rotary: sections or pair_axis, not both")
         if sections is not None:
             _need(sum(sections) == pairs and min(sections, default=0) >= 0,
@@ -68,7 +75,7 @@ class Rotary:
         _need(1 <= self.axes <= 4 and min(pair_axis, default=0) >= 0, "Rotary: 1 to 4 axes")
         for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
             if w is not None:
-                _dense(w, name, (w.numel(),), torch.float32, self.device)
+                _pointer(w, name, (w.numel(),), torch.float32, self.device)
         self.widths = {w.numel() for w in (q_weight, k_weight) if w is not None}
         self._keep = (cos, sin, q_weight, k_weight, (ctypes.c_uint8 * max(1, pairs))(*pair_axis))
         r = _lib.RotaryDesc()
@@ -91,10 +98,10 @@ class PagedCache:
         _need(isinstance(k_pages, torch.Tensor) and k_pages.is_cuda and k_pages.dim() == 4 and k_pages.dtype in FLOATS,
               "PagedCache: k_pages must be a CUDA tensor [num_pages, kv_heads, page_size, head_dim], f32, f16 or bf16")
         self.device, self.dtype = k_pages.device, k_pages.dtype
-        _dense(k_pages, "k_pages", k_pages.shape, self.dtype, self.device)
-        _dense(v_pages, "v_pages", k_pages.shape, self.dtype, self.device)
+        _pointer(k_pages, "k_pages", k_pages.shape, self.dtype, self.device)
+        _pointer(v_pages, "v_pages", k_pages.shape, self.dtype, self.device)
         _need(isinstance(page_table, torch.Tensor) and page_table.dim() == 2, "PagedCache: page_table must be [max_seqs, max_pages]")
-        _dense(page_table, "page_table", page_table.shape, torch.int32, self.device)
+        _pointer(page_table, "page_table", page_table.shape, torch.int32, self.device)
         self.k_pages, self.v_pages, self.page_table = k_pages, v_pages, page_table
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k_pages.shape
         self.max_seqs, self.max_pages = page_table.shape
@@ -108,6 +115,8 @@ class PagedCache:
         _lib.check(self._lib.tq4_paged_create(ctypes.byref(d), k_pages.data_ptr(), v_pages.data_ptr(),
                                               page_table.data_ptr(), self.device.index or 0, ctypes.byref(handle)))
         self._handle = handle
+        self._index = self.device.index or 0
+        self._scale = 1.0 / math.sqrt(self.head_dim)
         self._workspace = {}  # (heads, batch, with scores) -> bytes
 
     def close(self):
@@ -121,20 +130,20 @@ class PagedCache:
         except Exception:
             pass
 
-    def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
-
     def _rows(self, x, name, heads):
-        """x [tokens, heads, head_dim] with each token's heads contiguous; copied where they are not."""
-        _need(isinstance(x, torch.Tensor) and x.dim() == 3 and x.dtype == self.dtype and x.device == self.device
-              and x.shape[2] == self.head_dim and (heads is None or x.shape[1] == heads),
-              f"paged cache: {name} must be {self.dtype} [tokens, {heads or 'heads'}, {self.head_dim}] on {self.device}")
-        s = x.stride()
+        """x [tokens, heads, head_dim] with each token's heads contiguous, copied where they are not, and the
+        distance of its tokens."""
+        if not (isinstance(x, torch.Tensor) and x.dtype is self.dtype and x.device == self.device and x.dim() == 3
+                and x.shape[2] == self.head_dim and x.shape[1] == (heads or x.shape[1])):
+            raise ArgumentError(f"paged cache: {name} must be {self.dtype} [tokens, {heads or 'heads'}, {self.head_dim}] "
+                                f"on {self.device}")
         width = x.shape[1] * self.head_dim
-        if s[2] != 1 or (x.shape[1] > 1 and s[1] != self.head_dim) or (x.shape[0] > 1 and s[0] < width):
-            x = x.contiguous()
+        if not x.is_contiguous():
             s = x.stride()
-        return x, s[0] if x.shape[0] > 1 else width
+            if s[2] == 1 and (s[1] == self.head_dim or x.shape[1] == 1) and (s[0] >= width or x.shape[0] <= 1):
+                return x, max(s[0], width)
+            x = x.contiguous()
+        return x, width
 
     def append(self, q, k, v, seq, slot, positions=None, rotary=None, out=None):
         """Writes the keys and values of new tokens into the cache (token t is slot ``slot[t]`` of
@@ -142,34 +151,36 @@ class PagedCache:
         both normed and turned by ``rotary`` at ``positions`` (int32 [tokens], or [axes, tokens]).
         q [tokens, heads, head_dim], or None when only the cache is filled; k and v [tokens, kv_heads,
         head_dim]; views of a merged projection are read in place. ``out`` may not overlap q."""
+        device = self.device
         k, ks = self._rows(k, "k", self.kv_heads)
         v, vs = self._rows(v, "v", self.kv_heads)
         tokens = k.shape[0]
-        _need(v.shape[0] == tokens, f"paged cache: {v.shape[0]} values for {tokens} keys")
-        heads, qs = 0, 0
+        if v.shape[0] != tokens:
+            raise ArgumentError(f"paged cache: {v.shape[0]} values for {tokens} keys")
+        heads = qs = 0
+        q_p = out_p = pos_p = ref = None
         if q is not None:
             q, qs = self._rows(q, "q", None)
             heads = q.shape[1]
-            _need(q.shape[0] == tokens and heads > 0, f"paged cache: {q.shape[0]} queries for {tokens} keys")
+            if q.shape[0] != tokens or heads == 0:
+                raise ArgumentError(f"paged cache: {q.shape[0]} queries of {heads} heads for {tokens} keys")
+            q_p = q.data_ptr()
             if out is None:
-                out = torch.empty((tokens, heads, self.head_dim), dtype=self.dtype, device=self.device)
-            else:
-                _dense(out, "out", (tokens, heads, self.head_dim), self.dtype, self.device)
-        else:
-            _need(out is None, "paged cache: out without q")
-        seq_p = _dense(seq, "seq", (tokens,), torch.int32, self.device)
-        slot_p = _dense(slot, "slot", (tokens,), torch.int32, self.device)
-        pos_p = ref = None
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out_p = _pointer(out, "out", q.shape, self.dtype, device)
+        elif out is not None:
+            raise ArgumentError("paged cache: out without q")
+        seq_p = _pointer(seq, "seq", (tokens,), torch.int32, device)
+        slot_p = _pointer(slot, "slot", (tokens,), torch.int32, device)
         if rotary is not None:
-            _need(rotary.device == self.device and 2 * rotary.pairs <= self.head_dim and rotary.widths <= {self.head_dim},
-                  f"paged cache: the rotary embedding does not fit heads of {self.head_dim} values on {self.device}")
+            if rotary.device != device or 2 * rotary.pairs > self.head_dim or not rotary.widths <= {self.head_dim}:
+                raise ArgumentError(f"paged cache: the rotary embedding does not fit heads of {self.head_dim} values on {device}")
             ref = rotary._ref
             if rotary.pairs:
-                shape = (tokens,) if rotary.axes == 1 and positions is not None and positions.dim() == 1 else (rotary.axes, tokens)
-                pos_p = _dense(positions, "positions", shape, torch.int32, self.device)
-        _lib.check(self._lib.tq4_paged_append(
-            self._handle, q.data_ptr() if q is not None else None, qs, k.data_ptr(), ks, v.data_ptr(), vs, heads, tokens,
-            seq_p, slot_p, pos_p, ref, out.data_ptr() if out is not None else None, self._stream()))
+                flat = rotary.axes == 1 and isinstance(positions, torch.Tensor) and positions.dim() == 1
+                pos_p = _pointer(positions, "positions", (tokens,) if flat else (rotary.axes, tokens), torch.int32, device)
+        _lib.check(self._lib.tq4_paged_append(self._handle, q_p, qs, k.data_ptr(), ks, v.data_ptr(), vs, heads, tokens,
+                                              seq_p, slot_p, pos_p, ref, out_p, _raw_stream(self._index)))
         return out
 
     def attention(self, q, lengths, scale=None, window=0, scores=None, new_scores=None, out=None):
@@ -178,23 +189,24 @@ class PagedCache:
         head_dim]. Length 0 gives zeros; ``scale`` is 1 / sqrt(head_dim) by default. With ``scores``
         (f32 [batch, kv_heads, max_pages * page_size]) each slot's softmax weights, summed over the
         query heads of a KV head, are added to them: in place, or into ``new_scores``."""
+        device = self.device
         q, qs = self._rows(q, "q", None)
-        batch, heads = q.shape[:2]
-        _need(0 < heads and heads % self.kv_heads == 0,
-              f"paged cache: {heads} query heads are not a multiple of {self.kv_heads} KV heads")
-        _need(batch <= self.max_seqs, f"paged cache: {batch} sequences, the page table has {self.max_seqs}")
-        len_p = _dense(lengths, "lengths", (batch,), torch.int32, self.device)
-        in_p = out_p = None
+        batch, heads, _ = q.shape
+        if heads == 0 or heads % self.kv_heads:
+            raise ArgumentError(f"paged cache: {heads} query heads are not a multiple of {self.kv_heads} KV heads")
+        if batch > self.max_seqs:
+            raise ArgumentError(f"paged cache: {batch} sequences, the page table has {self.max_seqs}")
+        len_p = _pointer(lengths, "lengths", (batch,), torch.int32, device)
+        in_p = new_p = None
         if scores is not None:
             shape = (batch, self.kv_heads, self.max_slots)
-            in_p = _dense(scores, "scores", shape, torch.float32, self.device)
-            out_p = in_p if new_scores is None else _dense(new_scores, "new_scores", shape, torch.float32, self.device)
-        else:
-            _need(new_scores is None, "paged cache: new_scores without scores")
+            in_p = _pointer(scores, "scores", shape, torch.float32, device)
+            new_p = in_p if new_scores is None else _pointer(new_scores, "new_scores", shape, torch.float32, device)
+        elif new_scores is not None:
+            raise ArgumentError("paged cache: new_scores without scores")
         if out is None:
-            out = torch.empty((batch, heads, self.head_dim), dtype=self.dtype, device=self.device)
-        else:
-            _dense(out, "out", (batch, heads, self.head_dim), self.dtype, self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out_p = _pointer(out, "out", q.shape, self.dtype, device)
         key = (heads, batch, scores is not None)
         nbytes = self._workspace.get(key)
         if nbytes is None:
@@ -203,10 +215,10 @@ class PagedCache:
             nbytes = self._workspace[key] = n.value
         # a workspace of its own for each call, from torch's allocator: calls on several streams and
         # captured graphs never share one
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         _lib.check(self._lib.tq4_paged_attention(
-            self._handle, q.data_ptr(), qs, heads, len_p, batch, 1.0 / math.sqrt(self.head_dim) if scale is None else scale,
-            window, in_p, out_p, out.data_ptr(), ws.data_ptr(), nbytes, self._stream()))
+            self._handle, q.data_ptr(), qs, heads, len_p, batch, self._scale if scale is None else scale, window, in_p, new_p,
+            out_p, ws.data_ptr(), nbytes, _raw_stream(self._index)))
         return out
 
     def evict(self, lengths, scores, keep, recent, new_table, new_scores=None):
@@ -217,25 +229,23 @@ class PagedCache:
         new lengths int32 [batch]; the kept slots' scores). ``new_scores`` may be given, f32 [batch,
         kv_heads, keep or more]; a new one has 0 behind the kept slots and the width of the new table's
         slots, as ``attention`` over it wants."""
-        _need(isinstance(lengths, torch.Tensor) and lengths.dim() == 1, "paged cache: lengths must be int32 [batch]")
-        batch = lengths.shape[0]
-        _need(batch <= self.max_seqs, f"paged cache: {batch} sequences, the page table has {self.max_seqs}")
-        len_p = _dense(lengths, "lengths", (batch,), torch.int32, self.device)
-        score_p = _dense(scores, "scores", (batch, self.kv_heads, self.max_slots), torch.float32, self.device)
-        _need(isinstance(new_table, torch.Tensor) and new_table.dim() == 2, "paged cache: new_table must be int32 [batch, pages]")
-        pages = new_table.shape[1]
-        table_p = _dense(new_table, "new_table", (batch, pages), torch.int32, self.device)
+        device = self.device
+        batch = lengths.shape[0] if isinstance(lengths, torch.Tensor) and lengths.dim() == 1 else -1
+        if not 0 <= batch <= self.max_seqs:
+            raise ArgumentError(f"paged cache: lengths must be int32 [batch] of at most {self.max_seqs} sequences")
+        pages = new_table.shape[1] if isinstance(new_table, torch.Tensor) and new_table.dim() == 2 else -1
+        if not (0 <= recent <= keep and 0 < keep <= pages * self.page_size):
+            raise ArgumentError(f"paged cache: recent {recent} of keep {keep} slots, and a new_table [batch, pages] of int32 "
+                                f"with room for them on pages of {self.page_size}")
+        len_p = _pointer(lengths, "lengths", (batch,), torch.int32, device)
+        score_p = _pointer(scores, "scores", (batch, self.kv_heads, self.max_slots), torch.float32, device)
+        table_p = _pointer(new_table, "new_table", (batch, pages), torch.int32, device)
         if new_scores is None:
-            new_scores = torch.zeros((batch, self.kv_heads, max(keep, pages * self.page_size)), dtype=torch.float32, device=self.device)
-        else:
-            _need(isinstance(new_scores, torch.Tensor) and new_scores.dim() == 3 and new_scores.shape[2] >= keep,
-                  f"paged cache: new_scores must be f32 [batch, kv_heads, {keep} or more]")
-            _dense(new_scores, "new_scores", (batch, self.kv_heads, new_scores.shape[2]), torch.float32, self.device)
-        _need(0 <= recent <= keep and 0 < keep <= pages * self.page_size,
-              f"paged cache: recent {recent} of keep {keep} slots on {pages} pages of {self.page_size}")
-        kept = torch.empty((batch, self.kv_heads, keep), dtype=torch.int32, device=self.device)
-        new_lengths = torch.empty(batch, dtype=torch.int32, device=self.device)
-        _lib.check(self._lib.tq4_paged_evict(
-            self._handle, len_p, batch, score_p, keep, recent, table_p, pages, new_lengths.data_ptr(), kept.data_ptr(),
-            new_scores.data_ptr(), new_scores.shape[2], self._stream()))
+            new_scores = torch.zeros((batch, self.kv_heads, pages * self.page_size), dtype=torch.float32, device=device)
+        width = new_scores.shape[2] if isinstance(new_scores, torch.Tensor) and new_scores.dim() == 3 else 0
+        new_p = _pointer(new_scores, "new_scores", (batch, self.kv_heads, max(width, keep)), torch.float32, device)
+        kept = torch.empty((batch, self.kv_heads, keep), dtype=torch.int32, device=device)
+        new_lengths = torch.empty_like(lengths)
+        _lib.check(self._lib.tq4_paged_evict(self._handle, len_p, batch, score_p, keep, recent, table_p, pages,
+                                             new_lengths.data_ptr(), kept.data_ptr(), new_p, width, _raw_stream(self._index)))
         return kept, new_lengths, new_scores
