@@ -68,8 +68,8 @@ typedef struct {
  * q_out: token t is row slot[t] of sequence seq[t]. q [tokens][heads][head_dim], k and v
  * [tokens][kv_heads][head_dim], each token's heads contiguous and tokens `*_stride` values apart
  * (views of one merged projection); q_out is dense. positions is int32 [axes][tokens]. Norm and
- * rotation are computed in f32 and rounded once. seq[t] < 0 marks a padding token: nothing of it
- * is read or written, its row of q_out included. rotary may be NULL (no norm, no rotation;
+ * rotation are computed in f32 and rounded once. seq[t] < 0 marks a padding token: nothing is
+ * written for it, its row of q_out included. rotary may be NULL (no norm, no rotation;
  * positions unused), and q NULL with heads 0 (only the cache is filled). The (seq, slot) of two
  * tokens of a call must differ: which of the two would remain is not defined. q_out may not
  * overlap q. */

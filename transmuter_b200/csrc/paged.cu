@@ -1,6 +1,7 @@
 // The paged cache's handle, the write of new tokens into it (norm, rotary embedding, pages) and
 // eviction by accumulated attention weight (include/tq4_paged.h). Attention is paged_attention.cu.
 #include "paged.cuh"
+#include "sm100.cuh"
 
 namespace tq4 {
 
@@ -23,7 +24,154 @@ struct AppendArgs {
   uint8_t pair_axis[kAppendMaxPairs];
 };
 
-// A warp per row of a token: heads queries, then the keys, then the values.
+// Where token t goes: whether its numbers are all in range (else the status is set), its page, and the row in it.
+struct AppendPlace {
+  bool ok;
+  int page, in_page;
+  int64_t pos[4];
+};
+__device__ __forceinline__ AppendPlace append_place(const AppendArgs& a, int64_t t, int s, bool tell) {
+  const PagedView& c = a.cache;
+  AppendPlace p = {};
+  const int64_t slot = a.slot[t];
+  p.ok = s < c.max_seqs && slot >= 0 && slot < c.max_slots;
+  if (a.pairs > 0)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < a.axes) {
+        p.pos[i] = a.positions[i * a.tokens + t];
+        p.ok = p.ok && p.pos[i] >= 0 && p.pos[i] < a.max_pos;
+      }
+  p.page = p.ok ? c.table[(int64_t)s * c.max_pages + (slot >> c.page_log2)] : -1;
+  p.ok = c.page_ok(p.page);
+  if (!p.ok && tell) report(kDevBadArgument);
+  p.in_page = (int)(slot & ((1 << c.page_log2) - 1));
+  return p;
+}
+
+// Rows in 16-byte chunks. A lane has two chunks of a row whose values turn together: chunk u and the one half
+// the turned part further, or, interleaved, two neighbours; the unturned rest goes two chunks a lane too. So a
+// row is 1 << lpr lanes, and a warp's step takes 32 >> lpr rows of one token; it goes through `steps` of them
+// with the token's angles in registers. Memory bounds it: at 8191 tokens of 36 rows a row at a time (one value
+// a load, angles read again for every row) took 218 us, this takes AAA us.
+template <typename T>
+__global__ void __launch_bounds__(kAppendThreads) append_rows_kernel(const __grid_constant__ AppendArgs a, int lpr,
+                                                                    int steps, int warps_a_token) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int VE = 16 / sizeof(T);
+  const PagedView& c = a.cache;
+  const int lane = threadIdx.x & 31, D = c.head_dim, chunks = D / VE;
+  const int sub = lane & ((1 << lpr) - 1), group = lane >> lpr, rows_a_step = 32 >> lpr;
+  const int rows = a.heads + 2 * c.kv_heads, turned = a.heads + c.kv_heads;
+  const int64_t w = (int64_t)blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
+  const int64_t t = w / warps_a_token;
+  if (t >= a.tokens) return;
+  const int first = (int)(w - t * warps_a_token) * steps * rows_a_step + group;
+  const int half = a.interleaved ? 0 : a.pairs / VE;  // chunks to the partner
+  const int ca = sub < half ? sub : 2 * sub, cb = sub < half ? sub + half : ca + 1;
+  const bool has_a = ca < chunks, has_b = cb < chunks;
+
+  auto source = [&](int r) -> const T* {
+    if (r < a.heads) return static_cast<const T*>(a.q) + t * a.q_stride + (int64_t)r * D;
+    if (r < turned) return static_cast<const T*>(a.k) + t * a.k_stride + (int64_t)(r - a.heads) * D;
+    return static_cast<const T*>(a.v) + t * a.v_stride + (int64_t)(r - turned) * D;
+  };
+  uint4 xa = {}, xb = {};
+  auto load = [&](int r) {
+    if (r >= rows) return;
+    const T* x = source(r);
+    if (has_a) xa = *reinterpret_cast<const uint4*>(x + ca * VE);
+    if (has_b) xb = *reinterpret_cast<const uint4*>(x + cb * VE);
+  };
+  load(first);
+  const int s = a.seq[t];
+  if (s < 0) return;  // padding
+  const AppendPlace place = append_place(a, t, s, lane == 0);
+  if (!place.ok) return;
+  // the angles of this lane's pairs: VE of them
+  float cs[VE], sn[VE];
+  bool turn_a = false, turn_b = false;
+  if (a.interleaved) {
+    turn_a = has_a && ca * VE < 2 * a.pairs;
+    turn_b = has_b && cb * VE < 2 * a.pairs;
+  } else {
+    turn_a = turn_b = sub < half;
+  }
+  const int pair0 = a.interleaved ? ca * (VE / 2) : sub * VE;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    const bool on = a.interleaved ? (e < VE / 2 ? turn_a : turn_b) : turn_a;
+    cs[e] = 1.f;
+    sn[e] = 0.f;
+    if (on) {
+      const int i = pair0 + e, axis = a.pair_axis[i];
+      const int64_t row = (axis == 0 ? place.pos[0] : axis == 1 ? place.pos[1] : axis == 2 ? place.pos[2] : place.pos[3]) * a.pairs;
+      cs[e] = a.cos_t[row + i];
+      sn[e] = a.sin_t[row + i];
+    }
+  }
+  for (int step = 0; step < steps; ++step) {
+    const int r = first + step * rows_a_step;
+    uint4 ya = xa, yb = xb;
+    if (step + 1 < steps) load(r + rows_a_step);  // the next step's rows are on their way meanwhile
+    const bool key = r >= a.heads;
+    const float* nw = key ? a.k_w : a.q_w;
+    T* ea = reinterpret_cast<T*>(&ya);
+    T* eb = reinterpret_cast<T*>(&yb);
+    float fa[VE], fb[VE];
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      fa[e] = has_a ? to_f32(ea[e]) : 0.f;
+      fb[e] = has_b ? to_f32(eb[e]) : 0.f;
+      ss = fmaf(fb[e], fb[e], fmaf(fa[e], fa[e], ss));
+    }
+    for (int off = (1 << lpr) / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+    if (r < turned) {
+      if (nw) {
+        const float inv = 1.f / sqrtf(ss / (float)D + a.eps);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          if (has_a) fa[e] = fa[e] * inv * nw[ca * VE + e];
+          if (has_b) fb[e] = fb[e] * inv * nw[cb * VE + e];
+        }
+      }
+      if (a.interleaved) {
+#pragma unroll
+        for (int e = 0; e < VE / 2; ++e) {
+          const float x0 = fa[2 * e], x1 = fa[2 * e + 1], y0 = fb[2 * e], y1 = fb[2 * e + 1];
+          fa[2 * e] = x0 * cs[e] - x1 * sn[e];
+          fa[2 * e + 1] = x1 * cs[e] + x0 * sn[e];
+          fb[2 * e] = y0 * cs[VE / 2 + e] - y1 * sn[VE / 2 + e];
+          fb[2 * e + 1] = y1 * cs[VE / 2 + e] + y0 * sn[VE / 2 + e];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float x0 = fa[e], x1 = fb[e];
+          fa[e] = x0 * cs[e] - x1 * sn[e];
+          fb[e] = x1 * cs[e] + x0 * sn[e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        ea[e] = from_f32<T>(fa[e]);
+        eb[e] = from_f32<T>(fb[e]);
+      }
+    }
+    if (r >= rows) continue;
+    T* y;
+    if (!key) y = static_cast<T*>(a.q_out) + (t * a.heads + r) * D;
+    else if (r < turned) y = static_cast<T*>(a.k_pages) + c.row_offset(place.page, r - a.heads, place.in_page);
+    else y = static_cast<T*>(a.v_pages) + c.row_offset(place.page, r - turned, place.in_page);
+    if (has_a) *reinterpret_cast<uint4*>(y + ca * VE) = ya;
+    if (has_b) *reinterpret_cast<uint4*>(y + cb * VE) = yb;
+  }
+}
+
+// The same for what does not come in such chunks (views that start or step off 16 bytes, odd numbers of pairs):
+// a warp per row of a token, heads queries, then the keys, then the values.
 template <typename T>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
   pdl_wait();
@@ -37,20 +185,9 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
   if (t >= a.tokens) return;
   const int s = a.seq[t];
   if (s < 0) return;  // padding
-  const int64_t slot = a.slot[t];
-  bool ok = s < c.max_seqs && slot >= 0 && slot < c.max_slots;
-  int64_t pos[4] = {0, 0, 0, 0};
-  if (a.pairs > 0)
-    for (int i = 0; i < a.axes; ++i) {
-      pos[i] = a.positions[i * a.tokens + t];
-      ok = ok && pos[i] >= 0 && pos[i] < a.max_pos;
-    }
-  const int page = ok ? c.table[(int64_t)s * c.max_pages + (slot >> c.page_log2)] : -1;
-  if (!c.page_ok(page)) {
-    if (lane == 0) report(kDevBadArgument);
-    return;
-  }
-  const int in_page = (int)(slot & ((1 << c.page_log2) - 1));
+  const AppendPlace place = append_place(a, t, s, lane == 0);
+  if (!place.ok) return;
+  const int page = place.page, in_page = place.in_page;
   const T* x;
   T* y;
   const float* nw = nullptr;
@@ -87,7 +224,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
       x0 = x0 * inv * nw[e0];
       x1 = x1 * inv * nw[e1];
     }
-    const int64_t row = pos[a.pair_axis[i]] * pairs + i;
+    const int axis = a.pair_axis[i];
+    const int64_t row = (axis == 0 ? place.pos[0] : axis == 1 ? place.pos[1] : axis == 2 ? place.pos[2] : place.pos[3]) * pairs + i;
     const float cs = a.cos_t[row], sn = a.sin_t[row];
     y[e0] = from_f32<T>(x0 * cs - x1 * sn);
     y[e1] = from_f32<T>(x1 * cs + x0 * sn);
@@ -101,21 +239,21 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 }
 
 // ---- evict ------------------------------------------------------------------------------------
-constexpr int kSelectThreads = 1024;
-
 struct EvictArgs {
   PagedView cache;
   const int32_t* lengths;
   int64_t batch;
   const float* scores;
-  int64_t keep, recent;
+  int keep, recent;
   const int32_t* new_table;
   int32_t new_max_pages;
   int32_t *new_lengths, *kept;
   float* new_scores;
   int64_t new_score_stride;
   char *k_pages, *v_pages;
-  int row_bytes;
+  int row_bytes, chunk_shift;  // chunk_shift: log2 of a row's 16-byte chunks, or -1
+  int key_room;  // keys of its share that a CTA of the selection holds in shared memory
+  int move;      // the selection's CTAs move the rows too
 };
 
 // A score's place in the order: larger keys for larger scores, -0 as 0, NaN below all.
@@ -125,142 +263,320 @@ __device__ __forceinline__ uint32_t score_key(float f) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Sum over the threads before this one, and over all of them in *total (kSelectThreads threads).
-__device__ __forceinline__ int block_prefix(int v, int* warp_sums, int* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
-  for (int off = 1; off < 32; off <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, off);
-    if (lane >= off) x += y;
-  }
-  if (lane == 31) warp_sums[warp] = x;
-  __syncthreads();
-  if (warp == 0) {
-    int s = warp_sums[lane];
-    for (int off = 1; off < 32; off <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, s, off);
-      if (lane >= off) s += y;
+// Moves kept rows [j0, j1) of (sequence b, KV head h), by the block, kMoveRows at a time: threads look the rows'
+// places up, then all copy 16-byte chunks, kMoveAtOnce of K and of V in flight a thread.
+constexpr int kMoveRows = 64, kMoveAtOnce = 4;
+struct MoveRows {
+  int64_t from[kMoveRows], to[kMoveRows];  // bytes; from < 0: not to be moved
+};
+template <int THREADS>
+__device__ __forceinline__ void move_rows(const EvictArgs& a, int64_t b, int h, const int32_t* kept, int j0, int j1,
+                                          MoveRows& rows) {
+  const PagedView& c = a.cache;
+  const int mask = (1 << c.page_log2) - 1, chunks = a.row_bytes / 16, size = a.row_bytes / c.head_dim;
+  for (int base = j0; base < j1; base += kMoveRows) {
+    const int n = min(kMoveRows, j1 - base);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+      const int j = base + i, slot = kept[j];
+      int64_t from = -1, to = 0;
+      if (slot >= 0) {
+        const int p = c.table[b * c.max_pages + (slot >> c.page_log2)];
+        const int q = a.new_table[b * a.new_max_pages + (j >> c.page_log2)];
+        if (c.page_ok(p) && c.page_ok(q)) {
+          from = c.row_offset(p, h, slot & mask) * size;
+          to = c.row_offset(q, h, j & mask) * size;
+        } else {
+          report(kDevBadArgument);
+        }
+      }
+      rows.from[i] = from;
+      rows.to[i] = to;
     }
-    warp_sums[lane] = s;
+    __syncthreads();
+    for (int i0 = threadIdx.x; i0 < n * chunks; i0 += kMoveAtOnce * THREADS) {
+      uint4 k[kMoveAtOnce], v[kMoveAtOnce];
+      int64_t to[kMoveAtOnce];
+#pragma unroll
+      for (int m = 0; m < kMoveAtOnce; ++m) {
+        const int i = i0 + m * THREADS, row = a.chunk_shift >= 0 ? i >> a.chunk_shift : i / chunks;
+        to[m] = -1;
+        if (i < n * chunks && rows.from[row] >= 0) {
+          const int at = (i - row * chunks) * 16;
+          k[m] = *reinterpret_cast<const uint4*>(a.k_pages + rows.from[row] + at);
+          v[m] = *reinterpret_cast<const uint4*>(a.v_pages + rows.from[row] + at);
+          to[m] = rows.to[row] + at;
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < kMoveAtOnce; ++m)
+        if (to[m] >= 0) {
+          *reinterpret_cast<uint4*>(a.k_pages + to[m]) = k[m];
+          *reinterpret_cast<uint4*>(a.v_pages + to[m]) = v[m];
+        }
+    }
   }
-  __syncthreads();
-  const int before = warp ? warp_sums[warp - 1] : 0;
-  *total = warp_sums[31];
-  __syncthreads();
-  return before + x - v;
 }
 
-// One CTA per (sequence, KV head): the kept slots. The smallest kept score among the candidates is
-// found by radix selection, eight bits of the key a pass; then one ordered pass over the slots
-// takes the keys above it and the first of its equals.
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictArgs a) {
+constexpr int kBins = 2048;     // of a pass over 11 bits of the keys
+constexpr int kMaxCluster = 8;  // CTAs of a row
+
+// One cluster per (sequence, KV head): which slots are kept. A CTA has a share of the candidates, in shared memory
+// as keys. The smallest kept key is found by radix selection in three passes of 11, 11 and 10 bits: the
+// CTAs count their keys by digit, add up each other's counts through distributed shared memory, and each finds
+// the digit for itself. Then the keys above that one and the first of its equals are written out in order: a
+// warp has a run of the share, and ballots and sums of what lies before it give each key its place. One CTA a
+// row with four passes of 8 bits over global memory took BBB us for 16 rows of 131072 slots, this takes CCC us.
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_constant__ EvictArgs a) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ int hist[2][kBins];
+  __shared__ int warp_sums[WARPS];
+  __shared__ int counts[WARPS][2];  // keys above the edge and equal to it, of each warp
+  __shared__ int cta_counts[2];
+  __shared__ int s_digit, s_need;
+  __shared__ MoveRows rows;
+  extern __shared__ uint32_t keys[];
   pdl_wait();
   pdl_trigger();
-  __shared__ int hist[256];
-  __shared__ int warp_sums[32];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_need;
   const PagedView& c = a.cache;
-  const int64_t row = blockIdx.x;
+  const int C = (int)gridDim.x, rank = (int)blockIdx.x;
+  const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
   const int64_t b = row / c.kv_heads;
-  const int tid = threadIdx.x;
-  const int64_t L = paged_length(c, a.lengths, b);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const bool real = b < a.batch;  // the grid's last rows may not be; the same for a cluster
+  const int L = real ? (int)paged_length(c, a.lengths, b) : 0;
   const float* sc = a.scores + row * c.max_slots;
   int32_t* kept = a.kept + row * a.keep;
   float* ns = a.new_scores ? a.new_scores + row * a.new_score_stride : nullptr;
-  const int64_t stay = L < a.keep ? L : a.keep;
-  if (row == b * c.kv_heads && tid == 0) a.new_lengths[b] = (int32_t)stay;
-  for (int64_t i = stay + tid; i < a.keep; i += kSelectThreads) kept[i] = -1;
-  if (L <= a.keep) {
-    for (int64_t i = tid; i < L; i += kSelectThreads) {
-      kept[i] = (int32_t)i;
-      if (ns) ns[i] = sc[i];
-    }
-    return;
-  }
-  const int64_t n = L - a.recent;  // candidates, more than keep - recent of them
-  const int64_t most = a.keep - a.recent;
-  uint32_t edge = 0xffffffffu;
-  int need = 0;  // how many of the scores equal to the edge are kept
-  if (most > 0) {
-    uint32_t prefix = 0;
-    need = (int)most;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kSelectThreads) hist[i] = 0;
-      __syncthreads();
-      for (int64_t i = tid; i < n; i += kSelectThreads) {
-        const uint32_t key = score_key(sc[i]);
-        if (shift == 24 || ((key ^ prefix) >> (shift + 8)) == 0) atomicAdd(&hist[(key >> shift) & 255], 1);
+  const int stay = min(L, a.keep);
+  const int64_t all_threads = (int64_t)C * THREADS, me = (int64_t)rank * THREADS + tid;
+  if (real) {
+    if (row == b * c.kv_heads && me == 0) a.new_lengths[b] = stay;
+    for (int64_t i = stay + me; i < a.keep; i += all_threads) kept[i] = -1;
+    if (L <= a.keep) {
+      for (int64_t i = me; i < L; i += all_threads) {
+        kept[i] = (int32_t)i;
+        if (ns) ns[i] = sc[i];
       }
-      __syncthreads();
-      if (tid == 0) {
-        int d = 255, left = need;
-        while (d > 0 && hist[d] < left) left -= hist[d--];
-        s_prefix = prefix | ((uint32_t)d << shift);
-        s_need = left;
+    }
+  }
+  const int most = a.keep - a.recent;  // kept of the candidates
+  if (real && L > a.keep) {            // the same for a cluster
+    const int n = L - a.recent;        // candidates, more than `most`
+    for (int64_t i = me; i < a.recent; i += all_threads) {
+      kept[most + i] = (int32_t)(n + i);
+      if (ns) ns[most + i] = sc[n + i];
+    }
+    // this CTA's share
+    const int share = (n + C - 1) / C, lo = min(rank * share, n), m = min(share, n - lo);
+    const bool held = m <= a.key_room;
+    if (held && most > 0)
+      for (int i = tid; i < m; i += THREADS) keys[i] = score_key(sc[lo + i]);
+    auto key_at = [&](int i) { return held ? keys[i] : score_key(sc[lo + i]); };
+    uint32_t edge = 0xffffffffu;
+    int need = 0;  // how many of the keys equal to the edge are kept
+    if (most > 0) {
+      uint32_t prefix = 0;
+      need = most;
+      for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+        int* mine = hist[pass & 1];
+        for (int i = tid; i < kBins; i += THREADS) mine[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < m; i += THREADS) {
+          const uint32_t key = key_at(i);
+          if (pass == 0 || ((key ^ prefix) >> (pass == 1 ? 21 : 10)) == 0) atomicAdd(&mine[(key >> shift) & (bins - 1)], 1);
+        }
+        if (C > 1) cluster_sync_all();
+        else __syncthreads();
+        // bins from the top, a run of them a thread
+        constexpr int PER = kBins / THREADS;
+        int cnt[PER], sum = 0;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const int bin = kBins - 1 - (tid * PER + k);
+          int v = mine[bin];
+          if (C > 1) {
+            v = 0;
+            for (int r = 0; r < C; ++r) v += ld_cluster_s32(&mine[bin], (unsigned)r);
+          }
+          cnt[k] = v;
+          sum += v;
+        }
+        int incl = sum;
+        for (int off = 1; off < 32; off <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, incl, off);
+          if (lane >= off) incl += y;
+        }
+        if (lane == 31) warp_sums[warp] = incl;
+        __syncthreads();
+        int above = incl - sum;
+        for (int w = 0; w < warp; ++w) above += warp_sums[w];
+        if (above < need && above + sum >= need) {
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            if (above < need && above + cnt[k] >= need) {
+              s_digit = kBins - 1 - (tid * PER + k);
+              s_need = need - above;
+            }
+            above += cnt[k];
+          }
+        }
+        __syncthreads();
+        prefix |= (uint32_t)s_digit << shift;
+        need = s_need;
       }
-      __syncthreads();
-      prefix = s_prefix;
-      need = s_need;
-      __syncthreads();
+      edge = prefix;
     }
-    edge = prefix;
-  }
-  int64_t placed = 0, equals = 0;
-  for (int64_t base = 0; base < n && most > 0; base += kSelectThreads) {
-    const int64_t i = base + tid;
-    const float f = i < n ? sc[i] : 0.f;
-    const uint32_t key = score_key(f);
-    const bool eq = i < n && key == edge;
-    int total;
-    const int eq_before = block_prefix(eq, warp_sums, &total);
-    const bool take = i < n && (key > edge || (eq && equals + eq_before < need));
-    equals += total;
-    const int at = block_prefix(take, warp_sums, &total);
-    if (take) {
-      kept[placed + at] = (int32_t)i;
-      if (ns) ns[placed + at] = f;
+    // runs of the share, 32 keys at a time
+    const int run = ((m + WARPS - 1) / WARPS + 31) / 32 * 32, r0 = min(warp * run, m), r1 = min(r0 + run, m);
+    int above = 0, equal = 0;
+    for (int i0 = r0; i0 < r1 && most > 0; i0 += 32) {
+      const int i = i0 + lane;
+      const uint32_t key = i < r1 ? key_at(i) : 0;
+      above += __popc(__ballot_sync(0xffffffffu, i < r1 && key > edge));
+      equal += __popc(__ballot_sync(0xffffffffu, i < r1 && key == edge));
     }
-    placed += total;
+    if (lane == 0) {
+      counts[warp][0] = above;
+      counts[warp][1] = equal;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int x = 0, y = 0;
+      for (int w = 0; w < WARPS; ++w) {
+        x += counts[w][0];
+        y += counts[w][1];
+      }
+      cta_counts[0] = x;
+      cta_counts[1] = y;
+    }
+    if (C > 1) cluster_sync_all();
+    else __syncthreads();
+    int at = 0, equals = 0;  // kept, and equal to the edge, before this warp's run
+    for (int r = 0; r < rank; ++r) {
+      at += ld_cluster_s32(&cta_counts[0], (unsigned)r);
+      equals += ld_cluster_s32(&cta_counts[1], (unsigned)r);
+    }
+    for (int w = 0; w < warp; ++w) {
+      at += counts[w][0];
+      equals += counts[w][1];
+    }
+    at += min(equals, need);
+    for (int i0 = r0; i0 < r1 && most > 0; i0 += 32) {
+      const int i = i0 + lane;
+      const uint32_t key = i < r1 ? key_at(i) : 0;
+      const bool eq = i < r1 && key == edge;
+      const unsigned eqs = __ballot_sync(0xffffffffu, eq), before = (1u << lane) - 1;
+      const bool take = i < r1 && (key > edge || (eq && equals + __popc(eqs & before) < need));
+      const unsigned takes = __ballot_sync(0xffffffffu, take);
+      if (take) {
+        const int to = at + __popc(takes & before);
+        kept[to] = lo + i;
+        if (ns) ns[to] = sc[lo + i];
+      }
+      at += __popc(takes);
+      equals += __popc(eqs);
+    }
   }
-  for (int64_t i = tid; i < a.recent; i += kSelectThreads) {
-    kept[most + i] = (int32_t)(n + i);
-    if (ns) ns[most + i] = sc[n + i];
+  // no CTA leaves or goes on while another still reads its counts, or before all slots are written
+  if (C > 1) cluster_sync_all();
+  else __syncthreads();
+  if (a.move && real) {
+    const int per = (stay + C - 1) / C;
+    move_rows<THREADS>(a, b, (int)(row - b * c.kv_heads), kept, min(rank * per, stay), min((rank + 1) * per, stay), rows);
   }
 }
 
-// Moves the kept rows: a warp per row of K and V.
+// Moves the kept rows; gridDim.x blocks share a row's.
 constexpr int kMoveThreads = 256;
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictArgs a) {
+  __shared__ MoveRows rows;
   pdl_wait();
   pdl_trigger();
-  const PagedView& c = a.cache;
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = a.batch * c.kv_heads * a.keep;
-  for (int64_t w = (int64_t)blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5); w < rows;
-       w += (int64_t)gridDim.x * (kMoveThreads / 32)) {
-    const int64_t j = w % a.keep, bh = w / a.keep;
-    const int64_t b = bh / c.kv_heads;
-    const int h = (int)(bh - b * c.kv_heads);
-    const int slot = a.kept[w];
-    if (slot < 0) continue;
-    const int mask = (1 << c.page_log2) - 1;
-    const int from = c.table[b * c.max_pages + (slot >> c.page_log2)];
-    const int to = a.new_table[b * a.new_max_pages + (j >> c.page_log2)];
-    if (!c.page_ok(from) || !c.page_ok(to)) {
-      if (lane == 0) report(kDevBadArgument);
-      continue;
-    }
-    const int64_t size = a.row_bytes / c.head_dim;
-    const int64_t src = c.row_offset(from, h, slot & mask) * size, dst = c.row_offset(to, h, (int)(j & mask)) * size;
-    for (int i = lane * 16; i < a.row_bytes; i += 512) {
-      const uint4 k = *reinterpret_cast<const uint4*>(a.k_pages + src + i);
-      const uint4 v = *reinterpret_cast<const uint4*>(a.v_pages + src + i);
-      *reinterpret_cast<uint4*>(a.k_pages + dst + i) = k;
-      *reinterpret_cast<uint4*>(a.v_pages + dst + i) = v;
-    }
-  }
+  const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+  const int64_t b = row / a.cache.kv_heads;
+  if (b >= a.batch) return;
+  const int stay = a.new_lengths[b];
+  const int per = ((stay + (int)gridDim.x - 1) / (int)gridDim.x + 7) / 8 * 8;
+  const int j0 = min((int)blockIdx.x * per, stay);
+  move_rows<kMoveThreads>(a, b, (int)(row - b * a.cache.kv_heads), a.kept + row * a.keep, j0, min(j0 + per, stay), rows);
 }
+
+namespace {
+
+// Rows of up to this many bytes of K and V are moved by the selection's own CTAs: a launch less, but only as many
+// SMs as it has CTAs.
+constexpr int64_t kMoveInSelection = 4 << 20;
+
+template <typename T>
+tq4_status launch_append(const AppendArgs& a, cudaStream_t st) {
+  constexpr int VE = 16 / sizeof(T), kWarps = kAppendThreads / 32;
+  const int rows = a.heads + 2 * a.cache.kv_heads, chunks = a.cache.head_dim / VE;
+  const bool strides = a.q_stride % VE == 0 && a.k_stride % VE == 0 && a.v_stride % VE == 0;
+  if (strides && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.q_out) &&
+      (a.interleaved ? 2 * a.pairs : a.pairs) % VE == 0) {
+    const int half = a.interleaved ? 0 : a.pairs / VE, units = half + (chunks - 2 * half + 1) / 2;
+    int lpr = 0;
+    while ((1 << lpr) < units) ++lpr;  // units <= 32: head_dim <= 256
+    // few tokens are spread over the SMs, many go through a token's rows with its angles in registers
+    const int all = (rows + (32 >> lpr) - 1) / (32 >> lpr);
+    const int steps = (int)std::min<int64_t>(all, std::max<int64_t>(1, a.tokens * all / (148 * 64)));
+    const int warps = (all + steps - 1) / steps;
+    const int64_t blocks = (a.tokens * warps + kWarps - 1) / kWarps;
+    TQ4_CUDA(launch_pdl(append_rows_kernel<T>, dim3((unsigned)blocks), dim3(kAppendThreads), 0, st, a, lpr, steps, warps));
+    return TQ4_OK;
+  }
+  const int64_t blocks = (a.tokens * rows + kWarps - 1) / kWarps;
+  TQ4_CUDA(launch_pdl(append_kernel<T>, dim3((unsigned)blocks), dim3(kAppendThreads), 0, st, a));
+  return TQ4_OK;
+}
+
+template <int THREADS>
+tq4_status launch_select(const EvictArgs& a, dim3 grid, size_t smem, cudaStream_t st) {
+  static std::atomic<uint64_t> set{0};  // per device, per instantiation
+  TQ4_CUDA(set_smem_limit_once(evict_select_kernel<THREADS>, 200 * 1024, set));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = grid.x;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  TQ4_CUDA(cudaLaunchKernelEx(&cfg, evict_select_kernel<THREADS>, a));
+  return TQ4_OK;
+}
+
+tq4_status launch_evict(EvictArgs& a, int64_t rows, cudaStream_t st) {
+  const int64_t slots = a.cache.max_slots;
+  // a CTA has 8192 candidates at most where the cluster's size and the SMs allow it
+  int cluster = 1;
+  while (cluster < kMaxCluster && slots > (int64_t)cluster * 8192 && rows * cluster * 2 <= 148 * 2) cluster *= 2;
+  const int64_t share = (slots + cluster - 1) / cluster;
+  a.key_room = (int)std::min<int64_t>(share, 40 * 1024);
+  const unsigned y = (unsigned)std::min<int64_t>(rows, 65535), z = (unsigned)((rows + y - 1) / y);
+  const int64_t bytes = rows * a.keep * a.row_bytes * 2;
+  a.move = bytes <= kMoveInSelection;
+  const bool small = share <= 2048;
+  const size_t smem = (size_t)a.key_room * 4;
+  if (small) TQ4_TRY(launch_select<256>(a, dim3(cluster, y, z), smem, st));
+  else TQ4_TRY(launch_select<1024>(a, dim3(cluster, y, z), smem, st));
+  if (a.move) return TQ4_OK;
+  const int64_t tiles = (a.keep + kMoveRows - 1) / kMoveRows;
+  const unsigned blocks = (unsigned)std::min<int64_t>(tiles, std::max<int64_t>(1, 148 * 16 / rows));
+  TQ4_CUDA(launch_pdl(evict_move_kernel, dim3(blocks, y, z), dim3(kMoveThreads), 0, st, a));
+  return TQ4_OK;
+}
+
+}  // namespace
 
 }  // namespace tq4
 
@@ -401,15 +717,12 @@ tq4_status tq4_paged_append(const tq4_paged* cache, const void* q, int64_t q_str
     }
   }
   DeviceGuard guard(cache->device);
-  const int64_t warps = tokens * rows;
-  const dim3 grid((unsigned)((warps + kAppendThreads / 32 - 1) / (kAppendThreads / 32)));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (d.dtype) {
-    case TQ4_F16: TQ4_CUDA(launch_pdl(append_kernel<__half>, grid, dim3(kAppendThreads), 0, st, a)); break;
-    case TQ4_BF16: TQ4_CUDA(launch_pdl(append_kernel<__nv_bfloat16>, grid, dim3(kAppendThreads), 0, st, a)); break;
-    default: TQ4_CUDA(launch_pdl(append_kernel<float>, grid, dim3(kAppendThreads), 0, st, a)); break;
+    case TQ4_F16: return launch_append<__half>(a, st);
+    case TQ4_BF16: return launch_append<__nv_bfloat16>(a, st);
+    default: return launch_append<float>(a, st);
   }
-  return TQ4_OK;
 }
 
 tq4_status tq4_paged_evict(const tq4_paged* cache, const int32_t* lengths, int64_t batch, const float* scores,
@@ -458,8 +771,8 @@ tq4_status tq4_paged_evict(const tq4_paged* cache, const int32_t* lengths, int64
   a.lengths = lengths;
   a.batch = batch;
   a.scores = scores;
-  a.keep = keep;
-  a.recent = recent;
+  a.keep = (int)keep;
+  a.recent = (int)recent;
   a.new_table = new_table;
   a.new_max_pages = new_max_pages;
   a.new_lengths = new_lengths;
@@ -469,17 +782,15 @@ tq4_status tq4_paged_evict(const tq4_paged* cache, const int32_t* lengths, int64
   a.k_pages = static_cast<char*>(cache->k_pages);
   a.v_pages = static_cast<char*>(cache->v_pages);
   a.row_bytes = d.head_dim * dtype_size(d.dtype);
-  DeviceGuard guard(cache->device);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (rows > INT32_MAX) {
-    set_error("tq4_paged_evict: too many rows");
+  a.chunk_shift = -1;
+  for (int i = 0; i < 8; ++i)
+    if (a.row_bytes == 16 << i) a.chunk_shift = i;
+  if (rows > (int64_t)65535 * 65535) {
+    set_error("tq4_paged_evict: too many rows of sequences and KV heads");
     return TQ4_ERR_INVALID_ARGUMENT;
   }
-  TQ4_CUDA(launch_pdl(evict_select_kernel, dim3((unsigned)rows), dim3(kSelectThreads), 0, st, a));
-  const int64_t blocks = (rows * keep + kMoveThreads / 32 - 1) / (kMoveThreads / 32);
-  TQ4_CUDA(launch_pdl(evict_move_kernel, dim3((unsigned)std::min<int64_t>(blocks, 148 * 8)), dim3(kMoveThreads), 0, st,
-                      a));
-  return TQ4_OK;
+  DeviceGuard guard(cache->device);
+  return launch_evict(a, rows, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -116,6 +116,13 @@ __device__ __forceinline__ float ld_cluster_f32(const float* local, unsigned ran
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
   return v;
 }
+__device__ __forceinline__ int ld_cluster_s32(const int* local, unsigned rank) {
+  uint32_t addr = smem_u32(local), remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+  return v;
+}
 // 16 bytes of another cluster rank's shared memory at the address of `local` in this CTA's.
 __device__ __forceinline__ float4 ld_cluster_f32x4(const float* local, unsigned rank) {
   uint32_t addr = smem_u32(local), remote;
