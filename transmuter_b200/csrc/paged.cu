@@ -263,6 +263,10 @@ __device__ __forceinline__ uint32_t score_key(float f) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+__device__ __forceinline__ float key_score(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
+}
+
 // Moves kept rows [j0, j1) of (sequence b, KV head h), by the block, kMoveRows at a time: threads look the rows'
 // places up, then all copy 16-byte chunks, kMoveAtOnce of K and of V in flight a thread.
 constexpr int kMoveRows = 64, kMoveAtOnce = 4;
@@ -325,12 +329,13 @@ constexpr int kMaxCluster = 8;  // CTAs of a row
 // as keys. The smallest kept key is found by radix selection in three passes of 11, 11 and 10 bits: the
 // CTAs count their keys by digit, add up each other's counts through distributed shared memory, and each finds
 // the digit for itself. Then the keys above that one and the first of its equals are written out in order: a
-// warp has a run of the share, and ballots and sums of what lies before it give each key its place. One CTA a
+// thread has a run of the share, and the counts before it give each key its place. One CTA a
 // row with four passes of 8 bits over global memory took BBB us for 16 rows of 131072 slots, this takes CCC us.
 template <int THREADS>
-__global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_constant__ EvictArgs a) {
+__global__ void __launch_bounds__(THREADS, 2) evict_select_kernel(const __grid_constant__ EvictArgs a) {
   constexpr int WARPS = THREADS / 32;
-  __shared__ int hist[2][kBins];
+  __shared__ __align__(16) int hist[2][kBins];
+  __shared__ __align__(16) int sums[kBins];  // of the cluster's counts
   __shared__ int warp_sums[WARPS];
   __shared__ int counts[WARPS][2];  // keys above the edge and equal to it, of each warp
   __shared__ int cta_counts[2];
@@ -371,8 +376,17 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
     // this CTA's share
     const int share = (n + C - 1) / C, lo = min(rank * share, n), m = min(share, n - lo);
     const bool held = m <= a.key_room;
-    if (held && most > 0)
-      for (int i = tid; i < m; i += THREADS) keys[i] = score_key(sc[lo + i]);
+    if (held && most > 0) {
+      constexpr int kAtOnce = 8;  // loads in flight
+      for (int i0 = tid; i0 < m; i0 += kAtOnce * THREADS) {
+        float f[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) f[k] = i0 + k * THREADS < m ? sc[lo + i0 + k * THREADS] : 0.f;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k)
+          if (i0 + k * THREADS < m) keys[i0 + k * THREADS] = score_key(f[k]);
+      }
+    }
     auto key_at = [&](int i) { return held ? keys[i] : score_key(sc[lo + i]); };
     uint32_t edge = 0xffffffffu;
     int need = 0;  // how many of the keys equal to the edge are kept
@@ -390,19 +404,31 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
         }
         if (C > 1) cluster_sync_all();
         else __syncthreads();
+        const int* all = mine;
+        if (C > 1) {
+          for (int i = tid * 4; i < kBins; i += THREADS * 4) {
+            int4 v = make_int4(0, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r)
+              if (r < C) {
+                const float4 f = ld_cluster_f32x4(reinterpret_cast<const float*>(&mine[i]), (unsigned)r);
+                v.x += __float_as_int(f.x);
+                v.y += __float_as_int(f.y);
+                v.z += __float_as_int(f.z);
+                v.w += __float_as_int(f.w);
+              }
+            *reinterpret_cast<int4*>(&sums[i]) = v;
+          }
+          all = sums;
+          __syncthreads();
+        }
         // bins from the top, a run of them a thread
         constexpr int PER = kBins / THREADS;
         int cnt[PER], sum = 0;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-          const int bin = kBins - 1 - (tid * PER + k);
-          int v = mine[bin];
-          if (C > 1) {
-            v = 0;
-            for (int r = 0; r < C; ++r) v += ld_cluster_s32(&mine[bin], (unsigned)r);
-          }
-          cnt[k] = v;
-          sum += v;
+          cnt[k] = all[kBins - 1 - (tid * PER + k)];
+          sum += cnt[k];
         }
         int incl = sum;
         for (int off = 1; off < 32; off <<= 1) {
@@ -429,18 +455,25 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
       }
       edge = prefix;
     }
-    // runs of the share, 32 keys at a time
-    const int run = ((m + WARPS - 1) / WARPS + 31) / 32 * 32, r0 = min(warp * run, m), r1 = min(r0 + run, m);
+    // A thread has a run of the share, an odd number of keys, so that a warp's reads lie in different banks.
+    const int run = ((m + THREADS - 1) / THREADS) | 1, r0 = min(tid * run, m), r1 = most > 0 ? min(r0 + run, m) : r0;
     int above = 0, equal = 0;
-    for (int i0 = r0; i0 < r1 && most > 0; i0 += 32) {
-      const int i = i0 + lane;
-      const uint32_t key = i < r1 ? key_at(i) : 0;
-      above += __popc(__ballot_sync(0xffffffffu, i < r1 && key > edge));
-      equal += __popc(__ballot_sync(0xffffffffu, i < r1 && key == edge));
+    for (int i = r0; i < r1; ++i) {
+      const uint32_t key = key_at(i);
+      above += key > edge;
+      equal += key == edge;
     }
-    if (lane == 0) {
-      counts[warp][0] = above;
-      counts[warp][1] = equal;
+    int above_before = above, equal_before = equal;  // of the CTA's threads up to this one
+    for (int off = 1; off < 32; off <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, above_before, off), y = __shfl_up_sync(0xffffffffu, equal_before, off);
+      if (lane >= off) {
+        above_before += x;
+        equal_before += y;
+      }
+    }
+    if (lane == 31) {
+      counts[warp][0] = above_before;
+      counts[warp][1] = equal_before;
     }
     __syncthreads();
     if (tid == 0) {
@@ -454,30 +487,24 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
     }
     if (C > 1) cluster_sync_all();
     else __syncthreads();
-    int at = 0, equals = 0;  // kept, and equal to the edge, before this warp's run
-    for (int r = 0; r < rank; ++r) {
-      at += ld_cluster_s32(&cta_counts[0], (unsigned)r);
-      equals += ld_cluster_s32(&cta_counts[1], (unsigned)r);
-    }
+    int at = above_before - above, equals = equal_before - equal;  // before this thread's run, of all CTAs
     for (int w = 0; w < warp; ++w) {
       at += counts[w][0];
       equals += counts[w][1];
     }
-    at += min(equals, need);
-    for (int i0 = r0; i0 < r1 && most > 0; i0 += 32) {
-      const int i = i0 + lane;
-      const uint32_t key = i < r1 ? key_at(i) : 0;
-      const bool eq = i < r1 && key == edge;
-      const unsigned eqs = __ballot_sync(0xffffffffu, eq), before = (1u << lane) - 1;
-      const bool take = i < r1 && (key > edge || (eq && equals + __popc(eqs & before) < need));
-      const unsigned takes = __ballot_sync(0xffffffffu, take);
-      if (take) {
-        const int to = at + __popc(takes & before);
-        kept[to] = lo + i;
-        if (ns) ns[to] = sc[lo + i];
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r)
+      if (r < rank) {
+        at += ld_cluster_s32(&cta_counts[0], (unsigned)r);
+        equals += ld_cluster_s32(&cta_counts[1], (unsigned)r);
       }
-      at += __popc(takes);
-      equals += __popc(eqs);
+    at += min(equals, need);
+    for (int i = r0; i < r1; ++i) {
+      const uint32_t key = key_at(i);
+      if (key < edge || (key == edge && equals++ >= need)) continue;
+      kept[at] = lo + i;
+      if (ns) ns[at] = key == 0 || key == 0x80000000u ? sc[lo + i] : key_score(key);  // NaN and zeros have one key each
+      ++at;
     }
   }
   // no CTA leaves or goes on while another still reads its counts, or before all slots are written
@@ -568,7 +595,7 @@ tq4_status launch_evict(EvictArgs& a, int64_t rows, cudaStream_t st) {
   const bool small = share <= 2048;
   const size_t smem = (size_t)a.key_room * 4;
   if (small) TQ4_TRY(launch_select<256>(a, dim3(cluster, y, z), smem, st));
-  else TQ4_TRY(launch_select<1024>(a, dim3(cluster, y, z), smem, st));
+  else TQ4_TRY(launch_select<512>(a, dim3(cluster, y, z), smem, st));
   if (a.move) return TQ4_OK;
   const int64_t tiles = (a.keep + kMoveRows - 1) / kMoveRows;
   const unsigned blocks = (unsigned)std::min<int64_t>(tiles, std::max<int64_t>(1, 148 * 16 / rows));
