@@ -8,6 +8,7 @@ namespace tq4 {
 // ---- append -----------------------------------------------------------------------------------
 constexpr int kAppendThreads = 256;
 constexpr int kAppendMaxPairs = 128;  // head_dim <= 256
+constexpr int kAppendSteps = 4;      // rows of a lane, all of whose loads are in flight together
 
 struct AppendArgs {
   PagedView cache;
@@ -51,12 +52,12 @@ __device__ __forceinline__ AppendPlace append_place(const AppendArgs& a, int64_t
 
 // Rows in 16-byte chunks. A lane has two chunks of a row whose values turn together: chunk u and the one half
 // the turned part further, or, interleaved, two neighbours; the unturned rest goes two chunks a lane too. So a
-// row is 1 << lpr lanes, and a warp's step takes 32 >> lpr rows of one token; it goes through `steps` of them
-// with the token's angles in registers. Memory bounds it: at 8191 tokens of 36 rows a row at a time (one value
+// row is 1 << lpr lanes, and a warp's step takes 32 >> lpr rows of one token; its `steps` share the token's angles,
+// in registers. Memory bounds it: at 8191 tokens of 36 rows a row at a time (one value
 // a load, angles read again for every row) took 218 us, this takes AAA us.
 template <typename T>
-__global__ void __launch_bounds__(kAppendThreads) append_rows_kernel(const __grid_constant__ AppendArgs a, int lpr,
-                                                                    int steps, int warps_a_token) {
+__global__ void __launch_bounds__(kAppendThreads, 2) append_rows_kernel(const __grid_constant__ AppendArgs a, int lpr,
+                                                                       int steps, int warps_a_token) {
   pdl_wait();
   pdl_trigger();
   constexpr int VE = 16 / sizeof(T);
@@ -72,69 +73,101 @@ __global__ void __launch_bounds__(kAppendThreads) append_rows_kernel(const __gri
   const int ca = sub < half ? sub : 2 * sub, cb = sub < half ? sub + half : ca + 1;
   const bool has_a = ca < chunks, has_b = cb < chunks;
 
-  auto source = [&](int r) -> const T* {
-    if (r < a.heads) return static_cast<const T*>(a.q) + t * a.q_stride + (int64_t)r * D;
-    if (r < turned) return static_cast<const T*>(a.k) + t * a.k_stride + (int64_t)(r - a.heads) * D;
-    return static_cast<const T*>(a.v) + t * a.v_stride + (int64_t)(r - turned) * D;
-  };
-  uint4 xa = {}, xb = {};
-  auto load = [&](int r) {
-    if (r >= rows) return;
-    const T* x = source(r);
-    if (has_a) xa = *reinterpret_cast<const uint4*>(x + ca * VE);
-    if (has_b) xb = *reinterpret_cast<const uint4*>(x + cb * VE);
-  };
-  load(first);
+  uint4 xa[kAppendSteps], xb[kAppendSteps];
+#pragma unroll
+  for (int k = 0; k < kAppendSteps; ++k) {
+    const int r = first + k * rows_a_step;
+    xa[k] = xb[k] = make_uint4(0, 0, 0, 0);
+    if (k >= steps || r >= rows) continue;
+    const T* x = r < a.heads  ? static_cast<const T*>(a.q) + t * a.q_stride + (int64_t)r * D
+                 : r < turned ? static_cast<const T*>(a.k) + t * a.k_stride + (int64_t)(r - a.heads) * D
+                              : static_cast<const T*>(a.v) + t * a.v_stride + (int64_t)(r - turned) * D;
+    if (has_a) xa[k] = __ldg(reinterpret_cast<const uint4*>(x + ca * VE));
+    if (has_b) xb[k] = __ldg(reinterpret_cast<const uint4*>(x + cb * VE));
+  }
   const int s = a.seq[t];
   if (s < 0) return;  // padding
   const AppendPlace place = append_place(a, t, s, lane == 0);
   if (!place.ok) return;
   // the angles of this lane's pairs: VE of them
   float cs[VE], sn[VE];
-  bool turn_a = false, turn_b = false;
-  if (a.interleaved) {
-    turn_a = has_a && ca * VE < 2 * a.pairs;
-    turn_b = has_b && cb * VE < 2 * a.pairs;
-  } else {
-    turn_a = turn_b = sub < half;
-  }
+  const bool turn_a = a.interleaved ? has_a && ca * VE < 2 * a.pairs : sub < half;
+  const bool turn_b = a.interleaved ? has_b && cb * VE < 2 * a.pairs : turn_a;
   const int pair0 = a.interleaved ? ca * (VE / 2) : sub * VE;
+  const bool angles = first - group < turned;
+  if (angles && a.axes == 1) {  // rows of the tables in 16-byte pieces
 #pragma unroll
-  for (int e = 0; e < VE; ++e) {
-    const bool on = a.interleaved ? (e < VE / 2 ? turn_a : turn_b) : turn_a;
-    cs[e] = 1.f;
-    sn[e] = 0.f;
-    if (on) {
-      const int i = pair0 + e, axis = a.pair_axis[i];
-      const int64_t row = (axis == 0 ? place.pos[0] : axis == 1 ? place.pos[1] : axis == 2 ? place.pos[2] : place.pos[3]) * a.pairs;
-      cs[e] = a.cos_t[row + i];
-      sn[e] = a.sin_t[row + i];
+    for (int e = 0; e < VE; e += 4) {
+      float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (VE == 4 && a.interleaved) {  // the two chunks' pairs apart
+        const int64_t at = place.pos[0] * a.pairs + pair0;
+        if (turn_a) {
+          *reinterpret_cast<float2*>(&c4.x) = __ldg(reinterpret_cast<const float2*>(a.cos_t + at));
+          *reinterpret_cast<float2*>(&s4.x) = __ldg(reinterpret_cast<const float2*>(a.sin_t + at));
+        }
+        if (turn_b) {
+          *reinterpret_cast<float2*>(&c4.z) = __ldg(reinterpret_cast<const float2*>(a.cos_t + at + 2));
+          *reinterpret_cast<float2*>(&s4.z) = __ldg(reinterpret_cast<const float2*>(a.sin_t + at + 2));
+        }
+      } else if (!a.interleaved || e < VE / 2 ? turn_a : turn_b) {
+        const int64_t at = place.pos[0] * a.pairs + pair0 + e;
+        c4 = __ldg(reinterpret_cast<const float4*>(a.cos_t + at));
+        s4 = __ldg(reinterpret_cast<const float4*>(a.sin_t + at));
+      }
+      *reinterpret_cast<float4*>(cs + e) = c4;
+      *reinterpret_cast<float4*>(sn + e) = s4;
     }
-  }
-  for (int step = 0; step < steps; ++step) {
-    const int r = first + step * rows_a_step;
-    uint4 ya = xa, yb = xb;
-    if (step + 1 < steps) load(r + rows_a_step);  // the next step's rows are on their way meanwhile
-    const bool key = r >= a.heads;
-    const float* nw = key ? a.k_w : a.q_w;
-    T* ea = reinterpret_cast<T*>(&ya);
-    T* eb = reinterpret_cast<T*>(&yb);
-    float fa[VE], fb[VE];
-    float ss = 0.f;
+  } else {
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
-      fa[e] = has_a ? to_f32(ea[e]) : 0.f;
-      fb[e] = has_b ? to_f32(eb[e]) : 0.f;
-      ss = fmaf(fb[e], fb[e], fmaf(fa[e], fa[e], ss));
+      cs[e] = 1.f;
+      sn[e] = 0.f;
+      if (angles && (!a.interleaved || e < VE / 2 ? turn_a : turn_b)) {
+        const int i = pair0 + e, axis = a.pair_axis[i];
+        const int64_t row = (axis == 0 ? place.pos[0] : axis == 1 ? place.pos[1] : axis == 2 ? place.pos[2] : place.pos[3]) * a.pairs;
+        cs[e] = __ldg(a.cos_t + row + i);
+        sn[e] = __ldg(a.sin_t + row + i);
+      }
     }
-    for (int off = (1 << lpr) / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-    if (r < turned) {
-      if (nw) {
-        const float inv = 1.f / sqrtf(ss / (float)D + a.eps);
+  }
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          if (has_a) fa[e] = fa[e] * inv * nw[ca * VE + e];
-          if (has_b) fb[e] = fb[e] * inv * nw[cb * VE + e];
+  for (int k = 0; k < kAppendSteps; ++k) {
+    if (k >= steps) break;
+    const int r = first + k * rows_a_step;
+    T* ea = reinterpret_cast<T*>(&xa[k]);
+    T* eb = reinterpret_cast<T*>(&xb[k]);
+    if (r - group < turned) {  // the warp's rows are not all values
+      const float* nw = r < a.heads ? a.q_w : a.k_w;
+      float fa[VE], fb[VE];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        fa[e] = to_f32(ea[e]);  // chunks that are not there are zeros
+        fb[e] = to_f32(eb[e]);
+      }
+      if (a.q_w || a.k_w) {  // the same for the warp, whose rows may be of both
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) ss = fmaf(fb[e], fb[e], fmaf(fa[e], fa[e], ss));
+        for (int off = (1 << lpr) / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+        if (nw && r < turned) {
+          const float inv = 1.f / sqrtf(ss / (float)D + a.eps);
+#pragma unroll
+          for (int e = 0; e < VE; e += 4) {
+            if (has_a) {
+              const float4 w4 = __ldg(reinterpret_cast<const float4*>(nw + ca * VE + e));
+              fa[e] = fa[e] * inv * w4.x;
+              fa[e + 1] = fa[e + 1] * inv * w4.y;
+              fa[e + 2] = fa[e + 2] * inv * w4.z;
+              fa[e + 3] = fa[e + 3] * inv * w4.w;
+            }
+            if (has_b) {
+              const float4 w4 = __ldg(reinterpret_cast<const float4*>(nw + cb * VE + e));
+              fb[e] = fb[e] * inv * w4.x;
+              fb[e + 1] = fb[e + 1] * inv * w4.y;
+              fb[e + 2] = fb[e + 2] * inv * w4.z;
+              fb[e + 3] = fb[e + 3] * inv * w4.w;
+            }
+          }
         }
       }
       if (a.interleaved) {
@@ -154,19 +187,20 @@ __global__ void __launch_bounds__(kAppendThreads) append_rows_kernel(const __gri
           fb[e] = x1 * cs[e] + x0 * sn[e];
         }
       }
+      if (r < turned) {  // values stay as they are, bit for bit
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        ea[e] = from_f32<T>(fa[e]);
-        eb[e] = from_f32<T>(fb[e]);
+        for (int e = 0; e < VE; ++e) {
+          ea[e] = from_f32<T>(fa[e]);
+          eb[e] = from_f32<T>(fb[e]);
+        }
       }
     }
     if (r >= rows) continue;
-    T* y;
-    if (!key) y = static_cast<T*>(a.q_out) + (t * a.heads + r) * D;
-    else if (r < turned) y = static_cast<T*>(a.k_pages) + c.row_offset(place.page, r - a.heads, place.in_page);
-    else y = static_cast<T*>(a.v_pages) + c.row_offset(place.page, r - turned, place.in_page);
-    if (has_a) *reinterpret_cast<uint4*>(y + ca * VE) = ya;
-    if (has_b) *reinterpret_cast<uint4*>(y + cb * VE) = yb;
+    T* y = r < a.heads  ? static_cast<T*>(a.q_out) + (t * a.heads + r) * D
+           : r < turned ? static_cast<T*>(a.k_pages) + c.row_offset(place.page, r - a.heads, place.in_page)
+                        : static_cast<T*>(a.v_pages) + c.row_offset(place.page, r - turned, place.in_page);
+    if (has_a) *reinterpret_cast<uint4*>(y + ca * VE) = xa[k];
+    if (has_b) *reinterpret_cast<uint4*>(y + cb * VE) = xb[k];
   }
 }
 
@@ -542,15 +576,16 @@ tq4_status launch_append(const AppendArgs& a, cudaStream_t st) {
   constexpr int VE = 16 / sizeof(T), kWarps = kAppendThreads / 32;
   const int rows = a.heads + 2 * a.cache.kv_heads, chunks = a.cache.head_dim / VE;
   const bool strides = a.q_stride % VE == 0 && a.k_stride % VE == 0 && a.v_stride % VE == 0;
-  if (strides && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.q_out) &&
+  const bool tables = a.pairs % 4 == 0 && aligned16(a.cos_t) && aligned16(a.sin_t) && aligned16(a.q_w) && aligned16(a.k_w);
+  if (strides && tables && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.q_out) &&
       (a.interleaved ? 2 * a.pairs : a.pairs) % VE == 0) {
     const int half = a.interleaved ? 0 : a.pairs / VE, units = half + (chunks - 2 * half + 1) / 2;
     int lpr = 0;
     while ((1 << lpr) < units) ++lpr;  // units <= 32: head_dim <= 256
-    // few tokens are spread over the SMs, many go through a token's rows with its angles in registers
+    // few tokens are spread over the SMs
     const int all = (rows + (32 >> lpr) - 1) / (32 >> lpr);
-    const int steps = (int)std::min<int64_t>(all, std::max<int64_t>(1, a.tokens * all / (148 * 64)));
-    const int warps = (all + steps - 1) / steps;
+    const int most = (int)std::min<int64_t>(kAppendSteps, std::max<int64_t>(1, a.tokens * all / (148 * 16)));
+    const int warps = (all + most - 1) / most, steps = (all + warps - 1) / warps;
     const int64_t blocks = (a.tokens * warps + kWarps - 1) / kWarps;
     TQ4_CUDA(launch_pdl(append_rows_kernel<T>, dim3((unsigned)blocks), dim3(kAppendThreads), 0, st, a, lpr, steps, warps));
     return TQ4_OK;
