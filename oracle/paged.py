@@ -20,9 +20,10 @@ def place(table, page_size, seq, slot):
 def norm_rotate(x, w, eps, cos, sin, pair_axis, positions, interleaved):
     """One head's values [D] -> (normed and turned [D], f32 error bound [D]).
 
-    The sum of squares is a chain of at most 8 products a lane and 5 tree steps (13 u, halved by the
-    root), root, quotient and product by w add 4 u, and a turned value takes 3 roundings of terms
-    that together are at most sqrt(2) * hypot(pair): 20 u of the pair's length covers it."""
+    The sum of squares is a chain of at most 16 products a lane and 5 tree steps (with its mean 15 u or
+    fewer are met by a value; halved by the root), the reciprocal root is within 4 u, the products by
+    it and by w add 2 u, and a turned value takes 3 roundings of terms that together are at most
+    sqrt(2) * hypot(pair): 20 u of the pair's length covers it."""
     y = np.asarray(x, np.float64)
     if w is not None:
         y = y / math.sqrt(np.mean(y * y) + eps) * np.asarray(w, np.float64)

@@ -8,7 +8,7 @@ namespace tq4 {
 // ---- append -----------------------------------------------------------------------------------
 constexpr int kAppendThreads = 256;
 constexpr int kAppendMaxPairs = 128;  // head_dim <= 256
-constexpr int kAppendSteps = 4;      // rows of a lane, all of whose loads are in flight together
+constexpr int kAppendSteps = 3;      // rows of a lane, all of whose loads are in flight together
 
 struct AppendArgs {
   PagedView cache;
@@ -22,7 +22,7 @@ struct AppendArgs {
   int64_t max_pos;
   float eps;
   int pairs, axes, interleaved;
-  uint8_t pair_axis[kAppendMaxPairs];
+  uint32_t pair_axis[kAppendMaxPairs / 16];  // two bits a pair
 };
 
 // Where token t goes: whether its numbers are all in range (else the status is set), its page, and the row in it.
@@ -56,8 +56,8 @@ __device__ __forceinline__ AppendPlace append_place(const AppendArgs& a, int64_t
 // in registers. Memory bounds it: at 8191 tokens of 36 rows a row at a time (one value
 // a load, angles read again for every row) took 218 us, this takes AAA us.
 template <typename T>
-__global__ void __launch_bounds__(kAppendThreads, 2) append_rows_kernel(const __grid_constant__ AppendArgs a, int lpr,
-                                                                       int steps, int warps_a_token) {
+__global__ void __launch_bounds__(kAppendThreads, 3) append_rows_kernel(const __grid_constant__ AppendArgs a, int lpr,
+                                                                       int steps) {
   pdl_wait();
   pdl_trigger();
   constexpr int VE = 16 / sizeof(T);
@@ -65,23 +65,23 @@ __global__ void __launch_bounds__(kAppendThreads, 2) append_rows_kernel(const __
   const int lane = threadIdx.x & 31, D = c.head_dim, chunks = D / VE;
   const int sub = lane & ((1 << lpr) - 1), group = lane >> lpr, rows_a_step = 32 >> lpr;
   const int rows = a.heads + 2 * c.kv_heads, turned = a.heads + c.kv_heads;
-  const int64_t w = (int64_t)blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
-  const int64_t t = w / warps_a_token;
+  const int64_t t = (int64_t)blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
   if (t >= a.tokens) return;
-  const int first = (int)(w - t * warps_a_token) * steps * rows_a_step + group;
+  const int first = (int)blockIdx.y * steps * rows_a_step + group;
   const int half = a.interleaved ? 0 : a.pairs / VE;  // chunks to the partner
   const int ca = sub < half ? sub : 2 * sub, cb = sub < half ? sub + half : ca + 1;
   const bool has_a = ca < chunks, has_b = cb < chunks;
 
   uint4 xa[kAppendSteps], xb[kAppendSteps];
+  const T* q = static_cast<const T*>(a.q) + t * a.q_stride;
+  const T* kk = static_cast<const T*>(a.k) + t * a.k_stride;
+  const T* v = static_cast<const T*>(a.v) + t * a.v_stride;
 #pragma unroll
   for (int k = 0; k < kAppendSteps; ++k) {
     const int r = first + k * rows_a_step;
     xa[k] = xb[k] = make_uint4(0, 0, 0, 0);
     if (k >= steps || r >= rows) continue;
-    const T* x = r < a.heads  ? static_cast<const T*>(a.q) + t * a.q_stride + (int64_t)r * D
-                 : r < turned ? static_cast<const T*>(a.k) + t * a.k_stride + (int64_t)(r - a.heads) * D
-                              : static_cast<const T*>(a.v) + t * a.v_stride + (int64_t)(r - turned) * D;
+    const T* x = r < a.heads ? q + r * D : r < turned ? kk + (r - a.heads) * D : v + (r - turned) * D;
     if (has_a) xa[k] = __ldg(reinterpret_cast<const uint4*>(x + ca * VE));
     if (has_b) xb[k] = __ldg(reinterpret_cast<const uint4*>(x + cb * VE));
   }
@@ -90,67 +90,59 @@ __global__ void __launch_bounds__(kAppendThreads, 2) append_rows_kernel(const __
   const AppendPlace place = append_place(a, t, s, lane == 0);
   if (!place.ok) return;
   // the angles of this lane's pairs: VE of them
-  float cs[VE], sn[VE];
+  alignas(16) float cs[VE], sn[VE];
   const bool turn_a = a.interleaved ? has_a && ca * VE < 2 * a.pairs : sub < half;
   const bool turn_b = a.interleaved ? has_b && cb * VE < 2 * a.pairs : turn_a;
   const int pair0 = a.interleaved ? ca * (VE / 2) : sub * VE;
   const bool angles = first - group < turned;
-  if (angles && a.axes == 1) {  // rows of the tables in 16-byte pieces
+  // the axes of the lane's pairs; all in one word, since pair0 is a multiple of VE
+  const uint32_t axes = angles && pair0 < a.pairs ? a.pair_axis[pair0 / 16] >> (pair0 % 16 * 2) : 0;
+  auto table_row = [&](uint32_t axis) -> int64_t {
+    return (axis == 0 ? place.pos[0] : axis == 1 ? place.pos[1] : axis == 2 ? place.pos[2] : place.pos[3]) * a.pairs;
+  };
 #pragma unroll
-    for (int e = 0; e < VE; e += 4) {
-      float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (VE == 4 && a.interleaved) {  // the two chunks' pairs apart
-        const int64_t at = place.pos[0] * a.pairs + pair0;
-        if (turn_a) {
-          *reinterpret_cast<float2*>(&c4.x) = __ldg(reinterpret_cast<const float2*>(a.cos_t + at));
-          *reinterpret_cast<float2*>(&s4.x) = __ldg(reinterpret_cast<const float2*>(a.sin_t + at));
-        }
-        if (turn_b) {
-          *reinterpret_cast<float2*>(&c4.z) = __ldg(reinterpret_cast<const float2*>(a.cos_t + at + 2));
-          *reinterpret_cast<float2*>(&s4.z) = __ldg(reinterpret_cast<const float2*>(a.sin_t + at + 2));
-        }
-      } else if (!a.interleaved || e < VE / 2 ? turn_a : turn_b) {
-        const int64_t at = place.pos[0] * a.pairs + pair0 + e;
-        c4 = __ldg(reinterpret_cast<const float4*>(a.cos_t + at));
-        s4 = __ldg(reinterpret_cast<const float4*>(a.sin_t + at));
-      }
-      *reinterpret_cast<float4*>(cs + e) = c4;
-      *reinterpret_cast<float4*>(sn + e) = s4;
-    }
-  } else {
+  for (int e = 0; e < VE; e += 4) {
+    float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
+    const uint32_t four = (axes >> (2 * e)) & 255;
+    const bool on0 = angles && (!a.interleaved || e < VE / 2 ? turn_a : turn_b);
+    const bool on2 = angles && (!a.interleaved || e + 2 < VE / 2 ? turn_a : turn_b);  // of the upper two
+    if (on0 && on2 && four == (four & 3) * 0x55) {  // one axis: 16 bytes of a row of the tables
+      const int64_t at = table_row(four & 3) + pair0 + e;
+      c4 = __ldg(reinterpret_cast<const float4*>(a.cos_t + at));
+      s4 = __ldg(reinterpret_cast<const float4*>(a.sin_t + at));
+    } else {
 #pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      cs[e] = 1.f;
-      sn[e] = 0.f;
-      if (angles && (!a.interleaved || e < VE / 2 ? turn_a : turn_b)) {
-        const int i = pair0 + e, axis = a.pair_axis[i];
-        const int64_t row = (axis == 0 ? place.pos[0] : axis == 1 ? place.pos[1] : axis == 2 ? place.pos[2] : place.pos[3]) * a.pairs;
-        cs[e] = __ldg(a.cos_t + row + i);
-        sn[e] = __ldg(a.sin_t + row + i);
-      }
+      for (int i = 0; i < 4; ++i)
+        if (i < 2 ? on0 : on2) {
+          const int64_t at = table_row((four >> (2 * i)) & 3) + pair0 + e + i;
+          (&c4.x)[i] = __ldg(a.cos_t + at);
+          (&s4.x)[i] = __ldg(a.sin_t + at);
+        }
     }
+    *reinterpret_cast<float4*>(cs + e) = c4;
+    *reinterpret_cast<float4*>(sn + e) = s4;
   }
+  T* q_out = static_cast<T*>(a.q_out) + t * a.heads * D;
+  const int64_t at0 = c.row_offset(place.page, 0, place.in_page), head = (int64_t)D << c.page_log2;
+  T* k_out = static_cast<T*>(a.k_pages) + at0;
+  T* v_out = static_cast<T*>(a.v_pages) + at0;
+  const float inv_d = 1.f / (float)D;
 #pragma unroll
   for (int k = 0; k < kAppendSteps; ++k) {
     if (k >= steps) break;
     const int r = first + k * rows_a_step;
-    T* ea = reinterpret_cast<T*>(&xa[k]);
-    T* eb = reinterpret_cast<T*>(&xb[k]);
     if (r - group < turned) {  // the warp's rows are not all values
       const float* nw = r < a.heads ? a.q_w : a.k_w;
       float fa[VE], fb[VE];
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        fa[e] = to_f32(ea[e]);  // chunks that are not there are zeros
-        fb[e] = to_f32(eb[e]);
-      }
+      unpack16<T>(xa[k], fa);  // chunks that are not there are zeros
+      unpack16<T>(xb[k], fb);
       if (a.q_w || a.k_w) {  // the same for the warp, whose rows may be of both
         float ss = 0.f;
 #pragma unroll
         for (int e = 0; e < VE; ++e) ss = fmaf(fb[e], fb[e], fmaf(fa[e], fa[e], ss));
         for (int off = (1 << lpr) / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
         if (nw && r < turned) {
-          const float inv = 1.f / sqrtf(ss / (float)D + a.eps);
+          const float inv = rsqrtf(fmaf(ss, inv_d, a.eps));  // within 2^-22
 #pragma unroll
           for (int e = 0; e < VE; e += 4) {
             if (has_a) {
@@ -188,17 +180,12 @@ __global__ void __launch_bounds__(kAppendThreads, 2) append_rows_kernel(const __
         }
       }
       if (r < turned) {  // values stay as they are, bit for bit
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          ea[e] = from_f32<T>(fa[e]);
-          eb[e] = from_f32<T>(fb[e]);
-        }
+        xa[k] = pack16<T>(fa);
+        xb[k] = pack16<T>(fb);
       }
     }
     if (r >= rows) continue;
-    T* y = r < a.heads  ? static_cast<T*>(a.q_out) + (t * a.heads + r) * D
-           : r < turned ? static_cast<T*>(a.k_pages) + c.row_offset(place.page, r - a.heads, place.in_page)
-                        : static_cast<T*>(a.v_pages) + c.row_offset(place.page, r - turned, place.in_page);
+    T* y = r < a.heads ? q_out + r * D : r < turned ? k_out + (r - a.heads) * head : v_out + (r - turned) * head;
     if (has_a) *reinterpret_cast<uint4*>(y + ca * VE) = xa[k];
     if (has_b) *reinterpret_cast<uint4*>(y + cb * VE) = xb[k];
   }
@@ -258,7 +245,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
       x0 = x0 * inv * nw[e0];
       x1 = x1 * inv * nw[e1];
     }
-    const int axis = a.pair_axis[i];
+    const int axis = (a.pair_axis[i / 16] >> (i % 16 * 2)) & 3;
     const int64_t row = (axis == 0 ? place.pos[0] : axis == 1 ? place.pos[1] : axis == 2 ? place.pos[2] : place.pos[3]) * pairs + i;
     const float cs = a.cos_t[row], sn = a.sin_t[row];
     y[e0] = from_f32<T>(x0 * cs - x1 * sn);
@@ -586,8 +573,8 @@ tq4_status launch_append(const AppendArgs& a, cudaStream_t st) {
     const int all = (rows + (32 >> lpr) - 1) / (32 >> lpr);
     const int most = (int)std::min<int64_t>(kAppendSteps, std::max<int64_t>(1, a.tokens * all / (148 * 16)));
     const int warps = (all + most - 1) / most, steps = (all + warps - 1) / warps;
-    const int64_t blocks = (a.tokens * warps + kWarps - 1) / kWarps;
-    TQ4_CUDA(launch_pdl(append_rows_kernel<T>, dim3((unsigned)blocks), dim3(kAppendThreads), 0, st, a, lpr, steps, warps));
+    const dim3 grid((unsigned)((a.tokens + kWarps - 1) / kWarps), (unsigned)warps);
+    TQ4_CUDA(launch_pdl(append_rows_kernel<T>, grid, dim3(kAppendThreads), 0, st, a, lpr, steps));
     return TQ4_OK;
   }
   const int64_t blocks = (a.tokens * rows + kWarps - 1) / kWarps;
@@ -668,10 +655,10 @@ tq4_status tq4_paged_create(const tq4_paged_desc* desc, void* k_pages, void* v_p
     set_error("tq4_paged_create: page_size must be a power of two, got %d", d.page_size);
     return TQ4_ERR_INVALID_ARGUMENT;
   }
-  if (d.kv_heads <= 0 || d.num_pages <= 0 || d.num_pages > INT32_MAX || d.max_seqs <= 0 || d.max_pages <= 0 ||
+  if (d.kv_heads <= 0 || d.kv_heads > 16384 || d.num_pages <= 0 || d.num_pages > INT32_MAX || d.max_seqs <= 0 || d.max_pages <= 0 ||
       (int64_t)d.max_pages * d.page_size > ((int64_t)1 << 30) ||
       d.num_pages > ((int64_t)1 << 32) / d.page_size / d.kv_heads) {
-    set_error("tq4_paged_create: kv_heads, num_pages, max_seqs and max_pages must be positive, page numbers below "
+    set_error("tq4_paged_create: kv_heads (to 16384), num_pages, max_seqs and max_pages must be positive, page numbers below "
               "2^31, a sequence's slots (max_pages * page_size) at most 2^30, the pool's rows (num_pages * kv_heads * page_size) "
               "at most 2^32");
     return TQ4_ERR_INVALID_ARGUMENT;
@@ -712,8 +699,8 @@ tq4_status tq4_paged_append(const tq4_paged* cache, const void* q, int64_t q_str
   }
   const tq4_paged_desc& d = cache->desc;
   const int64_t rows = (int64_t)heads + 2 * (int64_t)d.kv_heads;
-  if (heads < 0 || (heads > 0) != (q != nullptr) || (q && !q_out)) {
-    set_error("tq4_paged_append: q and q_out with heads > 0, or neither with heads 0");
+  if (heads < 0 || heads > 65535 || (heads > 0) != (q != nullptr) || (q && !q_out)) {
+    set_error("tq4_paged_append: q and q_out with 1 to 65535 heads, or neither with heads 0");
     return TQ4_ERR_INVALID_ARGUMENT;
   }
   if (tokens < 0 || tokens > (int64_t)INT32_MAX * (kAppendThreads / 32) / rows) {
@@ -775,7 +762,7 @@ tq4_status tq4_paged_append(const tq4_paged* cache, const void* q, int64_t q_str
         set_error("tq4_paged_append: pair %d follows axis %d of %d", i, r.pair_axis[i], r.axes);
         return TQ4_ERR_INVALID_ARGUMENT;
       }
-      a.pair_axis[i] = r.pair_axis[i];
+      a.pair_axis[i / 16] |= (uint32_t)r.pair_axis[i] << (i % 16 * 2);
     }
   }
   DeviceGuard guard(cache->device);
