@@ -233,8 +233,17 @@ def check_attention(out, new, c, q, lengths, window, scores, scale=None):
         assert np.all(np.abs(f64(new) - want_new) <= new_bound), np.max(np.abs(f64(new) - want_new) - new_bound)
 
 
-def run_attention(dtype, heads, kv, d, ps, lengths, window, with_scores, seed=2, gain=2.0, scale=None):
-    k, v, table, _ = make_pool(lengths, kv, ps, d, dtype, seed, width=-(-max(lengths) // ps) + 2)
+# A page table with room for these sequences alone, and one for 40000 slots: few sequences of a tight table
+# are a cluster's each, those of a wide one share a line of work whatever their lengths.
+TABLES = pytest.mark.parametrize("wide", [False, True], ids=["tight", "wide"])
+
+
+def width_of(wide, lengths, ps):
+    return -(-(40000 if wide else max(lengths)) // ps) + 2
+
+
+def run_attention(dtype, heads, kv, d, ps, lengths, window, with_scores, seed=2, gain=2.0, scale=None, wide=False):
+    k, v, table, _ = make_pool(lengths, kv, ps, d, dtype, seed, width=width_of(wide, lengths, ps))
     c = paged.PagedCache(k, v, table)
     g = torch.Generator(DEV).manual_seed(seed)
     q = (torch.randn(len(lengths), heads, d, device=DEV, generator=g) * gain).to(dtype)
@@ -249,15 +258,17 @@ def run_attention(dtype, heads, kv, d, ps, lengths, window, with_scores, seed=2,
     return c, q, out
 
 
+@TABLES
 @pytest.mark.parametrize("case", ATTENTIONS, ids=str)
-def test_attention(case):
-    run_attention(*case)
+def test_attention(case, wide):
+    run_attention(*case, wide=wide)
 
 
+@TABLES
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("gain,scale", [(40.0, None), (1.0, 0.0), (2.0, -0.3), (1e-3, 2.0)])
-def test_attention_scales(dtype, gain, scale):
-    run_attention(dtype, 8, 2, 64, 16, [100, 1, 33], 0, True, gain=gain, scale=scale)
+def test_attention_scales(dtype, gain, scale, wide):
+    run_attention(dtype, 8, 2, 64, 16, [100, 1, 33], 0, True, gain=gain, scale=scale, wide=wide)
 
 
 @pytest.mark.parametrize("dtype,heads", [(F32, 4), (BF16, 4), (F16, 32)])
@@ -266,10 +277,11 @@ def test_attention_many_sequences(dtype, heads):
     run_attention(dtype, heads, 2, 16, 4, lengths, 0, True)
 
 
+@TABLES
 @pytest.mark.parametrize("dtype", [F32, F16])
-def test_attention_in_place_scores_and_strided_queries(dtype):
+def test_attention_in_place_scores_and_strided_queries(dtype, wide):
     lengths, kv, d = [50, 20], 2, 64
-    k, v, table, _ = make_pool(lengths, kv, 16, d, dtype, 5)
+    k, v, table, _ = make_pool(lengths, kv, 16, d, dtype, 5, width=width_of(wide, lengths, 16))
     c = paged.PagedCache(k, v, table)
     wide = torch.randn(2, 500, device=DEV).to(dtype)
     q = wide[:, 3:3 + 4 * d].unflatten(1, (4, d))
@@ -281,10 +293,11 @@ def test_attention_in_place_scores_and_strided_queries(dtype):
     check_attention(b, scores, c, q, lengths, 0, old)
 
 
+@TABLES
 @pytest.mark.parametrize("dtype", [F32, BF16])
-def test_attention_is_deterministic_and_independent_of_the_workspace(dtype):
+def test_attention_is_deterministic_and_independent_of_the_workspace(dtype, wide):
     lengths = [1500, 3, 700]
-    k, v, table, _ = make_pool(lengths, 2, 16, 128, dtype, 6)
+    k, v, table, _ = make_pool(lengths, 2, 16, 128, dtype, 6, width=width_of(wide, lengths, 16))
     c = paged.PagedCache(k, v, table)
     q = torch.randn(3, 8, 128, device=DEV).to(dtype)
     first = c.attention(q, ints(lengths))
@@ -304,9 +317,10 @@ def test_attention_shared_prefix_pages(dtype):
     check_attention(c.attention(q, ints([40, 33])), None, c, q, [40, 33], 0, None)
 
 
+@TABLES
 @pytest.mark.parametrize("dtype", [F32, BF16])
-def test_attention_flags_bad_lengths_and_pages(dtype):
-    k, v, table, _ = make_pool([20, 20, 20, 20], 2, 4, 64, dtype, 8)
+def test_attention_flags_bad_lengths_and_pages(dtype, wide):
+    k, v, table, _ = make_pool([20, 20, 20, 20], 2, 4, 64, dtype, 8, width=width_of(wide, [20], 4))
     c = paged.PagedCache(k, v, table)
     q = torch.randn(4, 4, 64, device=DEV).to(dtype)
     good = c.attention(q, ints([20, 20, 20, 20]))
@@ -325,10 +339,11 @@ def rest_rows(c, lo, hi):
     return paged.PagedCache(c.k_pages, c.v_pages, c.page_table[lo:hi].contiguous())
 
 
+@TABLES
 @pytest.mark.parametrize("dtype", [F32, F16])
-def test_attention_infinite_values_stay_in_their_rows(dtype):
+def test_attention_infinite_values_stay_in_their_rows(dtype, wide):
     """An infinite or NaN value in one sequence reaches no other."""
-    k, v, table, _ = make_pool([30, 30], 1, 16, 64, dtype, 9)
+    k, v, table, _ = make_pool([30, 30], 1, 16, 64, dtype, 9, width=width_of(wide, [30], 16))
     c = paged.PagedCache(k, v, table)
     q = torch.randn(2, 2, 64, device=DEV).to(dtype)
     good = c.attention(q, ints([30, 30]))
@@ -418,14 +433,15 @@ def test_attention_past_2_31_values():
     check_attention_long(c, q, [n], out, old, scores)
 
 
+@TABLES
 @pytest.mark.parametrize("dtype", [F32, BF16])
-def test_captured_step_replays_with_new_lengths(dtype):
+def test_captured_step_replays_with_new_lengths(dtype, wide):
     """Append and attention captured once; lengths, slots and pages change between replays, and two
     graphs replayed on two streams at once do not disturb each other."""
     kv, d, ps, heads = 2, 64, 16, 4
     states = []
     for seed in (1, 2):
-        k, v, table, _ = make_pool([90, 90], kv, ps, d, dtype, seed)
+        k, v, table, _ = make_pool([90, 90], kv, ps, d, dtype, seed, width=width_of(wide, [90], ps))
         c = paged.PagedCache(k, v, table)
         s = {"c": c, "q": torch.randn(2, heads, d, device=DEV).to(dtype), "k": torch.randn(2, kv, d, device=DEV).to(dtype),
              "v": torch.randn(2, kv, d, device=DEV).to(dtype), "len": ints([40, 7]), "slot": ints([39, 6]), "seq": ints([0, 1]),

@@ -63,6 +63,7 @@ struct AttnArgs {
   int tile, tiles;   // heads of a row, and rows of a KV head
   int unit, unit_log2;  // slots of a unit
   int warps, ctas, levels;  // of a CTA; CTAs the line is cut for; sizes of chunks at most
+  int cluster;              // CTAs of a row where there is no line, else 0
   int q_even;        // q's heads are 4-byte aligned
   float scale2;      // scale * log2(e): scores are kept for exp2
   const float* scores;
@@ -226,7 +227,6 @@ __device__ __forceinline__ int asked_cta(uint32_t from) {
   return got ? (int)x : -1;
 }
 
-// ---- part -----------------------------------------------------------------------------------------
 // A place in the line, stepped forward.
 struct Cursor {
   int b, r, u, units;
@@ -685,9 +685,89 @@ template <typename T, int DT, int TILE> constexpr int part_smem(int head_dim) {
                               (sizeof(T) == 4 ? TILE * head_dim * 4 + U * TILE * 4 : 0));
 }
 
+// Sends for a unit of KV head kvh, its keys and behind them its values, from slot p0 on. `page` is where lane i's
+// slot lies, or all of them (WHOLE). *valid gets a bit for each slot that counts; rows of others may hold
+// anything, NaN too, and become zeros.
+//
 // WHOLE: head_dim is DT and a page holds whole units. Then a unit's keys are one run of memory, as are its
 // values: one page lookup and constant offsets instead of one row address for each chunk (the loads of
 // a unit take 30 instructions a lane instead of 300).
+template <typename T, int DT, int U, bool WHOLE>
+__device__ __forceinline__ void load_rows(const AttnArgs& a, char* slot, uint32_t* valid, Span span, int p0, int kvh, int page) {
+  constexpr int VN = 16 / sizeof(T);
+  const PagedView& c = a.cache;
+  const int lane = threadIdx.x & 31, D = WHOLE ? DT : c.head_dim, chunks = D / VN, row_bytes = row_chunks<T>(D) * 16;
+  const int p = p0 + lane;
+  const bool in = lane < U && p >= span.lo && p < span.hi, ok = c.page_ok(page);
+  if (in && !ok) report(kDevBadArgument);
+  const uint32_t mask = __ballot_sync(0xffffffffu, in && ok);
+  if (lane == 0) *valid = mask;
+  const uint32_t dst = smem_u32(slot);
+  // a row's number in the pool: below 2^32 (checked by tq4_paged_create)
+  const uint32_t first = ((uint32_t)page * c.kv_heads + kvh) << c.page_log2;
+  const int in_page = (1 << c.page_log2) - 1;
+  if constexpr (WHOLE) {
+    constexpr int C = DT / VN, PITCH = row_chunks<T>(DT) * 16;
+    const int64_t off = (int64_t)(first + (p0 & in_page)) * (DT * (int)sizeof(T)) + lane * 16;
+    const char* kp = static_cast<const char*>(a.k_pages) + off;
+    const char* vp = static_cast<const char*>(a.v_pages) + off;
+    const uint32_t to = dst + (lane / C) * PITCH + (lane % C) * 16;
+    if (mask == (U == 32 ? 0xffffffffu : (1u << (U & 31)) - 1)) {
+#pragma unroll
+      for (int j = 0; j < U * C / 32; ++j) {
+        const int at_row = j * 32 / C * PITCH + j * 32 % C * 16;
+        cp_async16(to + at_row, kp + j * 512);
+        cp_async16(to + U * PITCH + at_row, vp + j * 512);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < U * C / 32; ++j) {
+        const int at_row = j * 32 / C * PITCH + j * 32 % C * 16;
+        const bool take = (mask >> (lane / C + j * 32 / C)) & 1;
+        cp_async16(to + at_row, take ? kp + j * 512 : a.k_pages, take);
+        cp_async16(to + U * PITCH + at_row, take ? vp + j * 512 : a.v_pages, take);
+      }
+    }
+  } else {
+    const int step_row = 32 / chunks, step_col = 32 % chunks;  // from a lane's chunk to its next
+    const uint32_t row = first + (p & in_page);
+    int i = lane / chunks, col = lane - i * chunks;
+    for (int n = 0; n < U * chunks; n += 32) {  // every lane the same number of turns
+      const int from = min(i, U - 1);
+      const uint32_t rw = __shfl_sync(0xffffffffu, row, from);
+      const bool take = (mask >> from) & 1;
+      const int64_t off = take ? (int64_t)rw * (D * (int)sizeof(T)) + col * 16 : 0;
+      if (i < U) {
+        cp_async16(dst + i * row_bytes + col * 16, static_cast<const char*>(a.k_pages) + off, take);
+        cp_async16(dst + (U + i) * row_bytes + col * 16, static_cast<const char*>(a.v_pages) + off, take);
+      }
+      i += step_row;
+      col += step_col;
+      if (col >= chunks) {
+        col -= chunks;
+        ++i;
+      }
+    }
+  }
+}
+// The page of the unit's slot p0 + lane, or of p0 (WHOLE); -1 outside the span.
+template <int U, bool WHOLE>
+__device__ __forceinline__ int look_up_page(const AttnArgs& a, int b, Span span, int p0) {
+  const int lane = threadIdx.x & 31, p = p0 + (WHOLE ? 0 : lane);
+  if (WHOLE || (lane < U && p >= span.lo && p < span.hi))
+    return a.cache.table[(int64_t)b * a.cache.max_pages + (p >> a.cache.page_log2)];
+  return -1;
+}
+// 16-bit rows of an odd number of 16-byte chunks: their last 16-value step reads one more, kept at zero.
+template <typename T>
+__device__ __forceinline__ void zero_tails(char* ring, int n_rows, int head_dim) {
+  const int chunks = head_dim * (int)sizeof(T) / 16;
+  if (sizeof(T) == 2 && (chunks & 1))
+    for (int i = threadIdx.x & 31; i < n_rows; i += 32)
+      *reinterpret_cast<uint4*>(ring + i * row_chunks<T>(head_dim) * 16 + chunks * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// ---- part -----------------------------------------------------------------------------------------
 template <typename T, int DT, int TILE, bool WHOLE>
 __global__ void __launch_bounds__(kWarpsOf<T, TILE> * 32, DT <= 128 ? 2 : 1)
     attention_part_kernel(const __grid_constant__ AttnArgs a) {
@@ -713,10 +793,7 @@ __global__ void __launch_bounds__(kWarpsOf<T, TILE> * 32, DT <= 128 ? 2 : 1)
   float* ps = qs + TILE * D;
   const int rows = c.kv_heads * a.tiles;
 
-  // 16-bit rows of an odd number of 16-byte chunks: their last 16-value step reads one more, kept at zero
-  if (sizeof(T) == 2 && (chunks & 1))
-    for (int i = lane; i < kStages * 2 * U; i += 32)
-      *reinterpret_cast<uint4*>(ring + i * row_bytes + chunks * 16) = make_uint4(0, 0, 0, 0);
+  zero_tails<T>(ring, kStages * 2 * U, D);
   if (tid == 0) {
     s_abort = 0;
     s_taken = WARPS;  // each warp has a piece of the first chunk
@@ -824,66 +901,11 @@ __global__ void __launch_bounds__(kWarpsOf<T, TILE> * 32, DT <= 128 ? 2 : 1)
     }
   };
   auto look_up = [&]() -> int {
-    if (load_left == 0) return -1;
-    const int p = unit_slot(a, next.span, next.u) + (WHOLE ? 0 : lane);
-    if (WHOLE || (lane < U && p >= next.span.lo && p < next.span.hi))
-      return c.table[(int64_t)next.b * c.max_pages + (p >> c.page_log2)];
-    return -1;
+    return load_left ? look_up_page<U, WHOLE>(a, next.b, next.span, unit_slot(a, next.span, next.u)) : -1;
   };
-  auto load_unit = [&](int stage, const Cursor& next, int page) {
-    const int p0 = unit_slot(a, next.span, next.u), kvh = next.r / a.tiles;
-    const int p = p0 + lane;
-    const bool in = lane < U && p >= next.span.lo && p < next.span.hi, ok = c.page_ok(page);
-    if (in && !ok) report(kDevBadArgument);
-    const uint32_t mask = __ballot_sync(0xffffffffu, in && ok);
-    if (lane == 0) valid_of[warp][stage] = mask;
-    const uint32_t dst = smem_u32(ring + stage * slot_bytes);
-    // a row's number in the pool: below 2^32 (checked by tq4_paged_create)
-    const uint32_t first = ((uint32_t)page * c.kv_heads + kvh) << c.page_log2;
-    const int in_page = (1 << c.page_log2) - 1;
-    if constexpr (WHOLE) {
-      constexpr int C = DT / VN, PITCH = row_chunks<T>(DT) * 16;
-      const int64_t off = (int64_t)(first + (p0 & in_page)) * (DT * (int)sizeof(T)) + lane * 16;
-      const char* kp = static_cast<const char*>(a.k_pages) + off;
-      const char* vp = static_cast<const char*>(a.v_pages) + off;
-      const uint32_t to = dst + (lane / C) * PITCH + (lane % C) * 16;
-      if (mask == (U == 32 ? 0xffffffffu : (1u << (U & 31)) - 1)) {
-#pragma unroll
-        for (int j = 0; j < U * C / 32; ++j) {
-          const int at_row = j * 32 / C * PITCH + j * 32 % C * 16;
-          cp_async16(to + at_row, kp + j * 512);
-          cp_async16(to + U * PITCH + at_row, vp + j * 512);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < U * C / 32; ++j) {
-          const int at_row = j * 32 / C * PITCH + j * 32 % C * 16;
-          const bool take = (mask >> (lane / C + j * 32 / C)) & 1;
-          cp_async16(to + at_row, take ? kp + j * 512 : a.k_pages, take);
-          cp_async16(to + U * PITCH + at_row, take ? vp + j * 512 : a.v_pages, take);
-        }
-      }
-    } else {
-      const int step_row = 32 / chunks, step_col = 32 % chunks;  // from a lane's chunk to its next
-      const uint32_t row = first + (p & in_page);
-      int i = lane / chunks, col = lane - i * chunks;
-      for (int n = 0; n < U * chunks; n += 32) {  // every lane the same number of turns
-        const int from = min(i, U - 1);
-        const uint32_t rw = __shfl_sync(0xffffffffu, row, from);
-        const bool take = (mask >> from) & 1;
-        const int64_t off = take ? (int64_t)rw * (D * (int)sizeof(T)) + col * 16 : 0;
-        if (i < U) {
-          cp_async16(dst + i * row_bytes + col * 16, static_cast<const char*>(a.k_pages) + off, take);
-          cp_async16(dst + (U + i) * row_bytes + col * 16, static_cast<const char*>(a.v_pages) + off, take);
-        }
-        i += step_row;
-        col += step_col;
-        if (col >= chunks) {
-          col -= chunks;
-          ++i;
-        }
-      }
-    }
+  auto load_unit = [&](int stage, const Cursor& at, int page) {
+    load_rows<T, DT, U, WHOLE>(a, ring + stage * slot_bytes, &valid_of[warp][stage], at.span,
+                               unit_slot(a, at.span, at.u), at.r / a.tiles, page);
   };
 
   // ---- folding ----
@@ -970,6 +992,147 @@ __global__ void __launch_bounds__(kWarpsOf<T, TILE> * 32, DT <= 128 ? 2 : 1)
   }
   cp_async_wait<0>();
   if (s_abort && s_ask) mbar_drain(smem_u32(&answered), s_answers & 1);  // an answer may still be on its way
+}
+
+// ---- short sequences: one kernel ------------------------------------------------------------------
+// A cluster of CTAs a row: its warps have a run of the row's units each, the CTAs join their warps' parts in shared
+// memory and then one another's through distributed shared memory, and each adds the weights of its own slots to
+// the scores. Where the page table has room for kClusterUnits units a warp at most, this is one launch and two
+// trips to memory after the lengths instead of two launches and six: DDD.
+constexpr int kMaxClusterCtas = 8;
+constexpr int kClusterUnits = 8;
+template <typename T, int DT, int TILE, bool WHOLE>
+__global__ void __launch_bounds__(kWarpsOf<T, TILE> * 32, DT <= 128 ? 2 : 1)
+    attention_cluster_kernel(const __grid_constant__ AttnArgs a) {
+  using Fold = FoldOf<T, DT, TILE>;
+  constexpr int U = Fold::U, WARPS = kWarpsOf<T, TILE>, THREADS = WARPS * 32;
+  constexpr int VN = 16 / sizeof(T);
+  __shared__ uint32_t valid_of[WARPS][kStages];
+  __shared__ __align__(8) float mls[WARPS][TILE][2];
+  __shared__ __align__(8) float cta_ml[TILE][2];
+  __shared__ float2 stats[TILE];  // m, 1 / l of the row
+  extern __shared__ __align__(16) char dyn[];
+  const PagedView& c = a.cache;
+  const int D = WHOLE ? DT : c.head_dim, tid = threadIdx.x, warp = tid >> 5;
+  const int chunks = D / VN, row_bytes = row_chunks<T>(D) * 16, slot_bytes = 2 * U * row_bytes;
+  char* ring = dyn + warp * kStages * slot_bytes;
+  float* qs = reinterpret_cast<float*>(dyn + WARPS * kStages * slot_bytes) + warp * TILE * (D + U);
+  float* ps = qs + TILE * D;
+  const int C = (int)gridDim.x, rank = (int)blockIdx.x, rows = c.kv_heads * a.tiles;
+  const int64_t row = blockIdx.y, b = row / rows;
+  const int r = (int)(row - b * rows), kvh = r / a.tiles, g0 = (r - kvh * a.tiles) * TILE;
+  const int G = min(TILE, a.group - g0), h0 = kvh * a.group + g0;
+  zero_tails<T>(ring, kStages * 2 * U, D);
+  __syncwarp();
+  pdl_wait();
+  pdl_trigger();
+  Fold fold;
+  fold.load_q(a, b, h0, G, qs);
+  const Span span = span_of(a, b);
+  const int units = units_of(a, span), w = rank * WARPS + warp, all = C * WARPS;
+  const int u0 = units * w / all, u1 = units * (w + 1) / all;
+  fold.begin();
+  int load = u0, page = -1;
+  auto look_up = [&](int u) { return u < u1 ? look_up_page<U, WHOLE>(a, (int)b, span, unit_slot(a, span, u)) : -1; };
+  auto send = [&](int stage, int pg) {
+    if (load < u1) {
+      load_rows<T, DT, U, WHOLE>(a, ring + stage * slot_bytes, &valid_of[warp][stage], span, unit_slot(a, span, load), kvh, pg);
+      ++load;
+    }
+    cp_async_commit();
+  };
+  static_assert(kStages == 3, "the first units' pages are looked up together");
+  {
+    const int page0 = look_up(u0), page1 = look_up(u0 + 1);
+    page = look_up(u0 + 2);
+    send(0, page0);
+    send(1, page1);
+  }
+  float* weights = a.new_scores ? a.weights + ((b * c.kv_heads + kvh) * c.max_slots) * a.group + g0 : nullptr;
+  for (int u = u0, stage = 0; u < u1; ++u) {
+    cp_async_wait<kStages - 2>();
+    __syncwarp();
+    send(stage == 0 ? kStages - 1 : stage - 1, page);
+    page = look_up(load);
+    const int p0 = unit_slot(a, span, u);
+    fold.template fold<WHOLE>(a, ring + stage * slot_bytes, valid_of[warp][stage], row_bytes,
+                              sizeof(T) == 2 ? (D + 15) / 16 : chunks, weights ? weights + (int64_t)p0 * a.group : nullptr,
+                              span.lo - p0, span.hi - p0, G, ps, qs);
+    stage = stage == kStages - 1 ? 0 : stage + 1;
+  }
+  // the warps' parts, each in its own ring
+  cp_async_wait<0>();
+  __syncwarp();
+  fold.end(nullptr, reinterpret_cast<float*>(ring), &mls[warp][0][0], 1, G, D);
+  __syncthreads();
+  float* joined = reinterpret_cast<float*>(ring - warp * kStages * slot_bytes + slot_bytes);  // in the first ring's second stage
+  for (int i = tid; i < G * D; i += THREADS) {
+    const int g = i / D;
+    float2 ml = make_float2(mls[0][g][0], mls[0][g][1]);
+#pragma unroll
+    for (int v = 1; v < WARPS; ++v) ml.x = fmaxf(ml.x, mls[v][g][0]);
+    const float f = ml.x == -INFINITY ? 0.f : ml.x;
+    float o = 0.f, l = 0.f;
+#pragma unroll
+    for (int v = 0; v < WARPS; ++v) {
+      const float e = ex2(mls[v][g][0] - f);
+      o = fmaf(e, reinterpret_cast<const float*>(dyn + v * kStages * slot_bytes)[i], o);
+      l = fmaf(e, mls[v][g][1], l);
+    }
+    joined[i] = o;
+    if (i == g * D) {
+      cta_ml[g][0] = ml.x;
+      cta_ml[g][1] = l;
+    }
+  }
+  cluster_sync_all();
+  for (int i = rank * THREADS + tid; i < G * D; i += C * THREADS) {
+    const int g = i / D;
+    float m[kMaxClusterCtas], l[kMaxClusterCtas], o[kMaxClusterCtas];
+#pragma unroll
+    for (int k = 0; k < kMaxClusterCtas; ++k)
+      if (k < C) {
+        m[k] = ld_cluster_f32(&cta_ml[g][0], (unsigned)k);
+        l[k] = ld_cluster_f32(&cta_ml[g][1], (unsigned)k);
+        o[k] = ld_cluster_f32(joined + i, (unsigned)k);
+      }
+    float M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kMaxClusterCtas; ++k)
+      if (k < C) M = fmaxf(M, m[k]);
+    const float f = M == -INFINITY ? 0.f : M;
+    float num = 0.f, den = 0.f;
+#pragma unroll
+    for (int k = 0; k < kMaxClusterCtas; ++k)
+      if (k < C) {
+        const float e = ex2(m[k] - f);
+        num = fmaf(e, o[k], num);
+        den = fmaf(e, l[k], den);
+      }
+    static_cast<T*>(a.out)[(b * a.heads + h0) * D + i] = from_f32<T>(den == 0.f ? 0.f : num / den);
+  }
+  if (a.new_scores) {  // the heads are one tile
+    if (tid < G) {
+      float M = -INFINITY, den = 0.f;
+      for (int k = 0; k < C; ++k) M = fmaxf(M, ld_cluster_f32(&cta_ml[tid][0], (unsigned)k));
+      const float f = M == -INFINITY ? 0.f : M;
+      for (int k = 0; k < C; ++k)
+        den = fmaf(ex2(ld_cluster_f32(&cta_ml[tid][0], (unsigned)k) - f), ld_cluster_f32(&cta_ml[tid][1], (unsigned)k), den);
+      stats[tid] = make_float2(f, den == 0.f ? 0.f : 1.f / den);
+    }
+    __syncthreads();
+    const float* old = a.scores + (b * c.kv_heads + kvh) * c.max_slots;
+    float* now = a.new_scores + (b * c.kv_heads + kvh) * c.max_slots;
+    if (now != old)  // slots before the window keep theirs
+      for (int p = rank * THREADS + tid; p < span.lo; p += C * THREADS) now[p] = old[p];
+    const int first = max(span.lo, unit_slot(a, span, units * rank / C)), last = min(span.hi, unit_slot(a, span, units * (rank + 1) / C));
+    for (int p = first + tid; p < last; p += THREADS) {
+      float sum = 0.f;
+      for (int g = 0; g < G; ++g) sum = fmaf(ex2(weights[(int64_t)p * a.group + g] - stats[g].x), stats[g].y, sum);
+      now[p] = old[p] + sum;
+    }
+  }
+  cluster_sync_all();  // no CTA leaves while another still reads its shared memory
 }
 
 // ---- finish ---------------------------------------------------------------------------------------
@@ -1268,12 +1431,51 @@ tq4_status check_attention(const tq4_paged* cache, int heads, int64_t batch) {
   return TQ4_OK;
 }
 
+// CTAs of a row for the cluster kernel; 0 where the line's kernels are to be used: rows that do not fill the SMs
+// twice over, with room in the page table for few units a warp, and all heads of a KV head in one row where
+// there are scores.
+int cluster_size(const AttnArgs& a) {
+  const int64_t rows = a.batch * a.cache.kv_heads * a.tiles;
+  int64_t slots = a.cache.max_slots;
+  if (a.window > 0) slots = std::min(slots, a.window + a.unit);
+  const int64_t units = (slots + a.unit - 1) / a.unit;
+  if (rows > a.ctas || (a.new_scores && a.tiles > 1)) return 0;
+  int c = 1;
+  while (c < kMaxClusterCtas && rows * c * 2 <= a.ctas && units > (int64_t)c * a.warps) c *= 2;
+  return units <= (int64_t)c * a.warps * kClusterUnits ? c : 0;
+}
+
+template <typename T, int DT, int TILE>
+tq4_status launch_cluster(const AttnArgs& a, int c, cudaStream_t st) {
+  const bool whole = a.cache.head_dim == DT && (1 << a.cache.page_log2) >= a.unit;
+  const auto kern = whole ? attention_cluster_kernel<T, DT, TILE, true> : attention_cluster_kernel<T, DT, TILE, false>;
+  static std::atomic<uint64_t> set[2];  // per device, per instantiation
+  TQ4_CUDA(set_smem_limit_once(kern, part_smem<T, DT, TILE>(DT), set[whole]));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(c, (unsigned)(a.batch * a.cache.kv_heads * a.tiles));
+  cfg.blockDim = dim3(a.warps * 32);
+  cfg.dynamicSmemBytes = part_smem<T, DT, TILE>(a.cache.head_dim);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = c;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  TQ4_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
+  return TQ4_OK;
+}
+
 template <typename T, int DT, int TILE>
 tq4_status launch_part(AttnArgs& a, int64_t grid, cudaStream_t st) {
   if (a.unit != FoldOf<T, DT, TILE>::U || a.warps != kWarpsOf<T, TILE>) {
     set_error("tq4_paged_attention: the call was cut for other kernels");
     return TQ4_ERR_UNSUPPORTED;
   }
+  if (a.cluster) return launch_cluster<T, DT, TILE>(a, a.cluster, st);
   const bool whole = a.cache.head_dim == DT && (1 << a.cache.page_log2) >= a.unit;
   const auto kern = whole ? attention_part_kernel<T, DT, TILE, true> : attention_part_kernel<T, DT, TILE, false>;
   static std::atomic<uint64_t> set[2];  // per device, per instantiation
@@ -1303,6 +1505,7 @@ tq4_status launch_attention(AttnArgs& a, int64_t grid, cudaStream_t st) {
     if (a.tile == 8) TQ4_TRY((launch_width<T, 8>(a, grid, st)));
     else TQ4_TRY((launch_width<T, 16>(a, grid, st)));
   }
+  if (a.cluster) return TQ4_OK;
   const auto finish = a.group % 4 == 0   ? attention_finish_kernel<T, 4>
                       : a.group % 2 == 0 ? attention_finish_kernel<T, 2>
                                          : attention_finish_kernel<T, 1>;
@@ -1391,6 +1594,7 @@ tq4_status tq4_paged_attention(const tq4_paged* cache, const void* q, int64_t q_
   a.pieces = (int)shape.grid * shape.warps;
   a.parts = reinterpret_cast<float*>(w + ws.parts);
   a.weights = reinterpret_cast<float*>(w + ws.weights);
+  a.cluster = cluster_size(a);
   if (batch * d.kv_heads * a.tiles > ((int64_t)1 << 30)) {
     set_error("tq4_paged_attention: more than 2^30 rows of sequences and KV heads");
     return TQ4_ERR_INVALID_ARGUMENT;
