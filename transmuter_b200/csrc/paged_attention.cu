@@ -504,6 +504,7 @@ struct FmaFold {
   static constexpr int SLICES = 32 / PG;   // lanes that share a slot's row
   static constexpr int KJ = (DT / 4 + SLICES - 1) / SLICES;  // chunks of a lane
   static constexpr int COLS = DT <= 128 ? 1 : 2;
+  static constexpr int HALVES = DT == 64 ? 2 : 1;  // rows of up to 16 chunks: each half of the warp has every other slot
   static constexpr int N = 4 * TILE;
   static constexpr int STEPS = PG == 2 ? 4 : 3;
   static constexpr int LEFT = (N >> STEPS) > 0 ? (N >> STEPS) : 1;             // sums a lane ends with
@@ -602,26 +603,27 @@ struct FmaFold {
     __syncwarp();
     const char* vs = ks + U * row_bytes;
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      alignas(16) float pg_[TILE];
+    for (int i = 0; i < U / HALVES; ++i) {
+      const int slot = HALVES == 1 ? i : 2 * i + (lane >> 4), chunk = HALVES == 1 ? lane : lane & 15;
+      alignas(16) float p[TILE];
       if constexpr (TILE >= 4) {
 #pragma unroll
         for (int g = 0; g < TILE; g += 4)
-          *reinterpret_cast<float4*>(pg_ + g) = *reinterpret_cast<const float4*>(ps + i * TILE + g);
+          *reinterpret_cast<float4*>(p + g) = *reinterpret_cast<const float4*>(ps + slot * TILE + g);
       } else {
 #pragma unroll
-        for (int g = 0; g < TILE; ++g) pg_[g] = ps[i * TILE + g];
+        for (int g = 0; g < TILE; ++g) p[g] = ps[slot * TILE + g];
       }
 #pragma unroll
       for (int j = 0; j < COLS; ++j)
-        if (lane + j * 32 < chunks) {
-          const float4 x = *reinterpret_cast<const float4*>(vs + i * row_bytes + (lane + j * 32) * 16);
+        if (chunk + j * 32 < chunks) {
+          const float4 x = *reinterpret_cast<const float4*>(vs + slot * row_bytes + (chunk + j * 32) * 16);
 #pragma unroll
           for (int g = 0; g < TILE; ++g) {
-            o[j][0][g] = fmaf(pg_[g], x.x, o[j][0][g]);
-            o[j][1][g] = fmaf(pg_[g], x.y, o[j][1][g]);
-            o[j][2][g] = fmaf(pg_[g], x.z, o[j][2][g]);
-            o[j][3][g] = fmaf(pg_[g], x.w, o[j][3][g]);
+            o[j][0][g] = fmaf(p[g], x.x, o[j][0][g]);
+            o[j][1][g] = fmaf(p[g], x.y, o[j][1][g]);
+            o[j][2][g] = fmaf(p[g], x.z, o[j][2][g]);
+            o[j][3][g] = fmaf(p[g], x.w, o[j][3][g]);
           }
         }
     }
@@ -652,6 +654,11 @@ struct FmaFold {
 #pragma unroll
     for (int off = 16 / TILE; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
     l *= 1.f / COPIES;
+    if constexpr (HALVES == 2)
+#pragma unroll
+      for (int g = 0; g < TILE; ++g)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[0][e][g] += __shfl_xor_sync(0xffffffffu, o[0][e][g], 16);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if ((lane & (32 / TILE - 1)) == 0 && (idx >> 2) < G)
       *reinterpret_cast<float2*>(ml + 2 * (idx >> 2) * (out ? 1 : pieces)) =
@@ -661,7 +668,7 @@ struct FmaFold {
       const float f = out ? __shfl_sync(0xffffffffu, inv, g * (32 / TILE)) : 1.f;
 #pragma unroll
       for (int j = 0; j < COLS; ++j)
-        if (g < G && (lane + j * 32) * 4 < D) {
+        if (g < G && (lane + j * 32) * 4 < D) {  // (with HALVES the first half has all columns)
           float* p = (out ? out + g * D : part + g * pieces * D) + (lane + j * 32) * 4;  // out may be aligned to 4 bytes only
           p[0] = o[j][0][g] * f;
           p[1] = o[j][1][g] * f;
@@ -730,8 +737,32 @@ __device__ __forceinline__ void load_rows(const AttnArgs& a, char* slot, uint32_
     }
   } else {
     const int step_row = 32 / chunks, step_col = 32 % chunks;  // from a lane's chunk to its next
-    const uint32_t row = first + (p & in_page);
     int i = lane / chunks, col = lane - i * chunks;
+    if ((1 << c.page_log2) >= U) {  // the unit is one run of memory here too
+      const uint32_t row0 = __shfl_sync(0xffffffffu, first, mask ? __ffs(mask) - 1 : 0) + (p0 & in_page);
+      const int64_t off = (int64_t)row0 * (D * (int)sizeof(T)) + lane * 16;
+      const char* kp = static_cast<const char*>(a.k_pages) + off;
+      const char* vp = static_cast<const char*>(a.v_pages) + off;
+      uint32_t to = dst + i * row_bytes + col * 16;
+      const int step = step_row * row_bytes + step_col * 16, wrap = row_bytes - chunks * 16;
+      for (int n = lane; n < U * chunks; n += 32) {
+        const bool take = (mask >> i) & 1;
+        cp_async16(to, take ? kp : a.k_pages, take);
+        cp_async16(to + U * row_bytes, take ? vp : a.v_pages, take);
+        kp += 512;
+        vp += 512;
+        to += step;
+        i += step_row;
+        col += step_col;
+        if (col >= chunks) {
+          col -= chunks;
+          to += wrap;
+          ++i;
+        }
+      }
+      return;
+    }
+    const uint32_t row = first + (p & in_page);
     for (int n = 0; n < U * chunks; n += 32) {  // every lane the same number of turns
       const int from = min(i, U - 1);
       const uint32_t rw = __shfl_sync(0xffffffffu, row, from);
