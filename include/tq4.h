@@ -167,8 +167,9 @@ tq4_status tq4_gather_rows(const tq4_weight* w, const int64_t* indices, int64_t 
 /* Reads and clears the device status word that bounded waits and device-side checks write.
  * Synchronizes the handle's device. *code = 0 when no kernel reported an error. Codes: 0x101-0x104
  * a tensor-core GEMM pipeline wait ran out, 0x105 a split-K counter was inconsistent, 0x106 a
- * peer's flag did not arrive (N-sharded calls), 0x107 a decode-attention copy, 0x108 the GEMV's
- * activation staging, 0x200 a device-side argument check (decoder positions).
+ * peer's flag did not arrive (N-sharded calls), 0x107 a wait of the decode or paged attention, 0x108
+ * the GEMV's activation staging, 0x200 a device-side argument check (decoder positions; lengths,
+ * slots, positions and page numbers of the paged cache).
  * Failure detection of the reference: test/support/hang_watchdog.exs:1-40 flags a call that makes
  * no progress; here every device wait gives up after a limit and reports instead. */
 tq4_status tq4_device_status(int device, int32_t* code);
