@@ -87,6 +87,13 @@ APPENDS = [
     (F16, 2, 1, 8, 4, 4, 1, False, False),
     (F16, 2, 1, 40, 4, 0, 1, False, True),
     (BF16, 40, 2, 64, 16, 10, 1, True, False),
+    # rows in chunks of 8 and 4 bytes, and of single values
+    (BF16, 9, 3, 72, 8, 36, 3, False, True),
+    (F16, 10, 1, 40, 8, 10, 1, False, True),
+    (F32, 4, 2, 72, 8, 18, 3, False, True),
+    (F16, 4, 2, 256, 4, 6, 2, False, True),
+    (BF16, 4, 2, 72, 4, 9, 2, True, True),
+    (F32, 4, 2, 12, 4, 5, 1, False, True),
 ]
 
 

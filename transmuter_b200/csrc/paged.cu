@@ -50,18 +50,33 @@ __device__ __forceinline__ AppendPlace append_place(const AppendArgs& a, int64_t
   return p;
 }
 
-// Rows in 16-byte chunks. A lane has two chunks of a row whose values turn together: chunk u and the one half
+template <int N> __device__ __forceinline__ void load_weights(float (&w)[N], const float* p) {
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    if (N % 4 == 0 && e % 4 == 0) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(p + e));
+      w[e] = v.x;
+      w[e + 1] = v.y;
+      w[e + 2] = v.z;
+      w[e + 3] = v.w;
+    } else if (N % 4 != 0) {
+      w[e] = __ldg(p + e);
+      w[e + 1] = __ldg(p + e + 1);
+    }
+  }
+}
+
+// Rows in chunks of VE values, 16 bytes or, where views or pairs do not fit those, 8 or 4. A lane has two chunks of a row whose values turn together: chunk u and the one half
 // the turned part further, or, interleaved, two neighbours; the unturned rest goes two chunks a lane too. So a
 // row is 1 << lpr lanes, and a warp's step takes 32 >> lpr rows of one token; its `steps` share the token's angles,
 // in registers. Memory bounds it, and near that the instructions: at 8191 tokens of 36 rows of 128 bf16 values,
 // normed, with three axes, a row a warp with one value a load took 218 us, chunks without the loads of all steps
 // in flight 75 us, this 45 us (3.4 TB/s; the bytes alone would take 24 us).
-template <typename T>
+template <typename T, int VE>
 __global__ void __launch_bounds__(kAppendThreads, 3) append_rows_kernel(const __grid_constant__ AppendArgs a, int lpr,
                                                                        int steps) {
   pdl_wait();
   pdl_trigger();
-  constexpr int VE = 16 / sizeof(T);
   const PagedView& c = a.cache;
   const int lane = threadIdx.x & 31, D = c.head_dim, chunks = D / VE;
   const int sub = lane & ((1 << lpr) - 1), group = lane >> lpr, rows_a_step = 32 >> lpr;
@@ -73,18 +88,19 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_rows_kernel(const __
   const int ca = sub < half ? sub : 2 * sub, cb = sub < half ? sub + half : ca + 1;
   const bool has_a = ca < chunks, has_b = cb < chunks;
 
-  uint4 xa[kAppendSteps], xb[kAppendSteps];
+  Packed<T, VE> xa[kAppendSteps], xb[kAppendSteps];
   const T* q = static_cast<const T*>(a.q) + t * a.q_stride;
   const T* kk = static_cast<const T*>(a.k) + t * a.k_stride;
   const T* v = static_cast<const T*>(a.v) + t * a.v_stride;
 #pragma unroll
   for (int k = 0; k < kAppendSteps; ++k) {
     const int r = first + k * rows_a_step;
-    xa[k] = xb[k] = make_uint4(0, 0, 0, 0);
+    xa[k].clear();
+    xb[k].clear();
     if (k >= steps || r >= rows) continue;
     const T* x = r < a.heads ? q + r * D : r < turned ? kk + (r - a.heads) * D : v + (r - turned) * D;
-    if (has_a) xa[k] = __ldg(reinterpret_cast<const uint4*>(x + ca * VE));
-    if (has_b) xb[k] = __ldg(reinterpret_cast<const uint4*>(x + cb * VE));
+    if (has_a) xa[k].load(x + ca * VE);
+    if (has_b) xb[k].load(x + cb * VE);
   }
   const int s = a.seq[t];
   if (s < 0) return;  // padding
@@ -101,27 +117,31 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_rows_kernel(const __
   auto table_row = [&](uint32_t axis) -> int64_t {
     return (axis == 0 ? place.pos[0] : axis == 1 ? place.pos[1] : axis == 2 ? place.pos[2] : place.pos[3]) * a.pairs;
   };
+  constexpr int kRun = VE < 4 ? VE : 4;  // pairs whose angles come in one load where they follow one axis
 #pragma unroll
-  for (int e = 0; e < VE; e += 4) {
-    float4 c4 = make_float4(1.f, 1.f, 1.f, 1.f), s4 = make_float4(0.f, 0.f, 0.f, 0.f);
-    const uint32_t four = (axes >> (2 * e)) & 255;
-    const bool on0 = angles && (!a.interleaved || e < VE / 2 ? turn_a : turn_b);
-    const bool on2 = angles && (!a.interleaved || e + 2 < VE / 2 ? turn_a : turn_b);  // of the upper two
-    if (on0 && on2 && four == (four & 3) * 0x55) {  // one axis: 16 bytes of a row of the tables
-      const int64_t at = table_row(four & 3) + pair0 + e;
-      c4 = __ldg(reinterpret_cast<const float4*>(a.cos_t + at));
-      s4 = __ldg(reinterpret_cast<const float4*>(a.sin_t + at));
+  for (int e = 0; e < VE; e += kRun) {
+    bool on = angles, one = true;  // all of the run turn; all follow one axis
+    const uint32_t axis0 = (axes >> (2 * e)) & 3;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      on = on && (!a.interleaved || e + i < VE / 2 ? turn_a : turn_b);
+      one = one && ((axes >> (2 * (e + i))) & 3) == axis0;
+      cs[e + i] = 1.f;
+      sn[e + i] = 0.f;
+    }
+    if (kRun == 4 && on && one) {
+      const int64_t at = table_row(axis0) + pair0 + e;
+      *reinterpret_cast<float4*>(cs + e) = __ldg(reinterpret_cast<const float4*>(a.cos_t + at));
+      *reinterpret_cast<float4*>(sn + e) = __ldg(reinterpret_cast<const float4*>(a.sin_t + at));
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < 2 ? on0 : on2) {
-          const int64_t at = table_row((four >> (2 * i)) & 3) + pair0 + e + i;
-          (&c4.x)[i] = __ldg(a.cos_t + at);
-          (&s4.x)[i] = __ldg(a.sin_t + at);
+      for (int i = 0; i < kRun; ++i)
+        if (angles && (!a.interleaved || e + i < VE / 2 ? turn_a : turn_b)) {
+          const int64_t at = table_row((axes >> (2 * (e + i))) & 3) + pair0 + e + i;
+          cs[e + i] = __ldg(a.cos_t + at);
+          sn[e + i] = __ldg(a.sin_t + at);
         }
     }
-    *reinterpret_cast<float4*>(cs + e) = c4;
-    *reinterpret_cast<float4*>(sn + e) = s4;
   }
   T* q_out = static_cast<T*>(a.q_out) + t * a.heads * D;
   const int64_t at0 = c.row_offset(place.page, 0, place.in_page), head = (int64_t)D << c.page_log2;
@@ -135,8 +155,8 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_rows_kernel(const __
     if (r - group < turned) {  // the warp's rows are not all values
       const float* nw = r < a.heads ? a.q_w : a.k_w;
       float fa[VE], fb[VE];
-      unpack16<T>(xa[k], fa);  // chunks that are not there are zeros
-      unpack16<T>(xb[k], fb);
+      xa[k].get(fa);  // chunks that are not there are zeros
+      xb[k].get(fb);
       if (a.q_w || a.k_w) {  // the same for the warp, whose rows may be of both
         float ss = 0.f;
 #pragma unroll
@@ -144,22 +164,16 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_rows_kernel(const __
         for (int off = (1 << lpr) / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
         if (nw && r < turned) {
           const float inv = rsqrtf(fmaf(ss, inv_d, a.eps));  // within 2^-22
+          float w[VE];
+          if (has_a) {
+            load_weights<VE>(w, nw + ca * VE);
 #pragma unroll
-          for (int e = 0; e < VE; e += 4) {
-            if (has_a) {
-              const float4 w4 = __ldg(reinterpret_cast<const float4*>(nw + ca * VE + e));
-              fa[e] = fa[e] * inv * w4.x;
-              fa[e + 1] = fa[e + 1] * inv * w4.y;
-              fa[e + 2] = fa[e + 2] * inv * w4.z;
-              fa[e + 3] = fa[e + 3] * inv * w4.w;
-            }
-            if (has_b) {
-              const float4 w4 = __ldg(reinterpret_cast<const float4*>(nw + cb * VE + e));
-              fb[e] = fb[e] * inv * w4.x;
-              fb[e + 1] = fb[e + 1] * inv * w4.y;
-              fb[e + 2] = fb[e + 2] * inv * w4.z;
-              fb[e + 3] = fb[e + 3] * inv * w4.w;
-            }
+            for (int e = 0; e < VE; ++e) fa[e] = fa[e] * inv * w[e];
+          }
+          if (has_b) {
+            load_weights<VE>(w, nw + cb * VE);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) fb[e] = fb[e] * inv * w[e];
           }
         }
       }
@@ -181,18 +195,18 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_rows_kernel(const __
         }
       }
       if (r < turned) {  // values stay as they are, bit for bit
-        xa[k] = pack16<T>(fa);
-        xb[k] = pack16<T>(fb);
+        xa[k].set(fa);
+        xb[k].set(fb);
       }
     }
     if (r >= rows) continue;
     T* y = r < a.heads ? q_out + r * D : r < turned ? k_out + (r - a.heads) * head : v_out + (r - turned) * head;
-    if (has_a) *reinterpret_cast<uint4*>(y + ca * VE) = xa[k];
-    if (has_b) *reinterpret_cast<uint4*>(y + cb * VE) = xb[k];
+    if (has_a) xa[k].store(y + ca * VE);
+    if (has_b) xb[k].store(y + cb * VE);
   }
 }
 
-// The same for what does not come in such chunks (views that start or step off 16 bytes, odd numbers of pairs):
+// The same for what does not come in such chunks (16-bit views that start off 4 bytes, odd numbers of pairs):
 // a warp per row of a token, heads queries, then the keys, then the values.
 template <typename T>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
@@ -562,25 +576,43 @@ namespace {
 // short sequence, with the selection's other steps), but only as many SMs as it has CTAs.
 constexpr int64_t kMoveInSelection = 4 << 20;
 
+// Whether the rows come in chunks of VE values (*taken), and the launch if so.
+template <typename T, int VE>
+tq4_status launch_append_rows(const AppendArgs& a, cudaStream_t st, bool* taken) {
+  constexpr int kWarps = kAppendThreads / 32;
+  const int rows = a.heads + 2 * a.cache.kv_heads, chunks = a.cache.head_dim / VE;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
+                       reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.q_out);
+  const bool strides = a.q_stride % VE == 0 && a.k_stride % VE == 0 && a.v_stride % VE == 0;
+  // angles and norm weights in 16-byte loads
+  const bool tables = VE < 4 || (a.pairs % 4 == 0 && aligned16(a.cos_t) && aligned16(a.sin_t) && aligned16(a.q_w) && aligned16(a.k_w));
+  const int half = a.interleaved ? 0 : a.pairs / VE, units = half + (chunks - 2 * half + 1) / 2;
+  *taken = at % (VE * sizeof(T)) == 0 && strides && tables && (a.interleaved ? 2 * a.pairs : a.pairs) % VE == 0 && units <= 32;
+  if (!*taken) return TQ4_OK;
+  int lpr = 0;
+  while ((1 << lpr) < units) ++lpr;
+  // few tokens are spread over the SMs
+  const int all = (rows + (32 >> lpr) - 1) / (32 >> lpr);
+  const int most = (int)std::min<int64_t>(kAppendSteps, std::max<int64_t>(1, a.tokens * all / (148 * 16)));
+  const int warps = (all + most - 1) / most, steps = (all + warps - 1) / warps;
+  const dim3 grid((unsigned)((a.tokens + kWarps - 1) / kWarps), (unsigned)warps);
+  TQ4_CUDA(launch_pdl(append_rows_kernel<T, VE>, grid, dim3(kAppendThreads), 0, st, a, lpr, steps));
+  return TQ4_OK;
+}
+
 template <typename T>
 tq4_status launch_append(const AppendArgs& a, cudaStream_t st) {
-  constexpr int VE = 16 / sizeof(T), kWarps = kAppendThreads / 32;
-  const int rows = a.heads + 2 * a.cache.kv_heads, chunks = a.cache.head_dim / VE;
-  const bool strides = a.q_stride % VE == 0 && a.k_stride % VE == 0 && a.v_stride % VE == 0;
-  const bool tables = a.pairs % 4 == 0 && aligned16(a.cos_t) && aligned16(a.sin_t) && aligned16(a.q_w) && aligned16(a.k_w);
-  if (strides && tables && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.q_out) &&
-      (a.interleaved ? 2 * a.pairs : a.pairs) % VE == 0) {
-    const int half = a.interleaved ? 0 : a.pairs / VE, units = half + (chunks - 2 * half + 1) / 2;
-    int lpr = 0;
-    while ((1 << lpr) < units) ++lpr;  // units <= 32: head_dim <= 256
-    // few tokens are spread over the SMs
-    const int all = (rows + (32 >> lpr) - 1) / (32 >> lpr);
-    const int most = (int)std::min<int64_t>(kAppendSteps, std::max<int64_t>(1, a.tokens * all / (148 * 16)));
-    const int warps = (all + most - 1) / most, steps = (all + warps - 1) / warps;
-    const dim3 grid((unsigned)((a.tokens + kWarps - 1) / kWarps), (unsigned)warps);
-    TQ4_CUDA(launch_pdl(append_rows_kernel<T>, grid, dim3(kAppendThreads), 0, st, a, lpr, steps));
-    return TQ4_OK;
+  constexpr int kWarps = kAppendThreads / 32;
+  const int rows = a.heads + 2 * a.cache.kv_heads;
+  bool taken = false;
+  if constexpr (sizeof(T) == 2) {
+    TQ4_TRY((launch_append_rows<T, 8>(a, st, &taken)));
+    if (taken) return TQ4_OK;
   }
+  TQ4_TRY((launch_append_rows<T, 4>(a, st, &taken)));
+  if (taken) return TQ4_OK;
+  TQ4_TRY((launch_append_rows<T, 2>(a, st, &taken)));
+  if (taken) return TQ4_OK;
   const int64_t blocks = (a.tokens * rows + kWarps - 1) / kWarps;
   TQ4_CUDA(launch_pdl(append_kernel<T>, dim3((unsigned)blocks), dim3(kAppendThreads), 0, st, a));
   return TQ4_OK;

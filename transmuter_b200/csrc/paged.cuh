@@ -69,26 +69,40 @@ template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t x) {
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t x) {
   return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
 }
-// The values of a 16-byte chunk, and back.
-template <typename T> __device__ __forceinline__ void unpack16(const uint4& x, float (&f)[16 / sizeof(T)]) {
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+// N values of a type in 4, 8 or 16 bytes, as they are loaded and stored.
+template <typename T, int N> struct Packed {
+  static constexpr int kWords = N * (int)sizeof(T) / 4;
+  using Raw = std::conditional_t<kWords == 4, uint4, std::conditional_t<kWords == 2, uint2, uint32_t>>;
+  union {
+    Raw raw;
+    uint32_t w[kWords];
+  };
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(T) == 4) {
-      f[i] = __uint_as_float(w[i]);
-    } else {
-      const float2 v = unpack2<T>(w[i]);
-      f[2 * i] = v.x;
-      f[2 * i + 1] = v.y;
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  __device__ __forceinline__ void load(const T* p) { raw = __ldg(reinterpret_cast<const Raw*>(p)); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = raw; }
+  __device__ __forceinline__ void get(float (&f)[N]) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        f[i] = __uint_as_float(w[i]);
+      } else {
+        const float2 v = unpack2<T>(w[i]);
+        f[2 * i] = v.x;
+        f[2 * i + 1] = v.y;
+      }
     }
   }
-}
-template <typename T> __device__ __forceinline__ uint4 pack16(const float (&f)[16 / sizeof(T)]) {
-  if constexpr (sizeof(T) == 4)
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-  else
-    return make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
-}
+  __device__ __forceinline__ void set(const float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
+      else w[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
+    }
+  }
+};
 
 // The length of sequence b, 0 (and the device status set) where it cannot be one.
 __device__ __forceinline__ int64_t paged_length(const PagedView& c, const int32_t* lengths, int64_t b) {
