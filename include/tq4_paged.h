@@ -72,7 +72,7 @@ typedef struct {
  * written for it, its row of q_out included. rotary may be NULL (no norm, no rotation;
  * positions unused), and q NULL with heads 0 (only the cache is filled). The (seq, slot) of two
  * tokens of a call must differ: which of the two would remain is not defined. q_out may not
- * overlap q. */
+ * overlap q, k or v. */
 tq4_status tq4_paged_append(const tq4_paged* cache, const void* q, int64_t q_stride, const void* k,
                             int64_t k_stride, const void* v, int64_t v_stride, int heads,
                             int64_t tokens, const int32_t* seq, const int32_t* slot,
@@ -88,7 +88,7 @@ tq4_status tq4_paged_attention_workspace(const tq4_paged* cache, int heads, int6
  * over the rows of KV head h / (heads / kv_heads) of sequence b = row b of the page table, the new
  * token's own row among them (append it first). window = 0 attends to the whole sequence. A
  * sequence of length 0 gives zeros, and so does a head whose every score is -inf. q is [batch][heads][head_dim], rows q_stride values apart; out
- * is dense. heads is any multiple of kv_heads.
+ * is dense and may not overlap q. heads is any multiple of kv_heads.
  * With scores and new_scores (f32 [batch][kv_heads][max_pages * page_size], both or neither; they
  * may be the same buffer), the softmax weights that eviction goes by are accumulated: slot j of
  * new_scores is that of scores plus the sum over the KV head's query heads of slot j's weight, and
@@ -108,9 +108,9 @@ tq4_status tq4_paged_attention(const tq4_paged* cache, const void* q, int64_t q_
  * new_table[b] (int32 [batch][new_max_pages]); kept [batch][kv_heads][keep] tells the old slots
  * (-1 behind the last), new_lengths [batch] the new lengths, and new_scores, if not NULL, takes the
  * scores along (rows new_score_stride >= keep values apart; what lies behind is left as it was).
- * The pages of new_table are pages of the same pool that no sequence of this call lists in its
- * page table: the old rows are only read, so that pages shared with other sequences stay whole. No
- * output may overlap an input. */
+ * The pages of new_table are pages of the same pool, each in one place of it, that no sequence of
+ * this call lists in its page table: the old rows are only read, so that pages shared with other
+ * sequences stay whole. No output may overlap an input or another output. */
 tq4_status tq4_paged_evict(const tq4_paged* cache, const int32_t* lengths, int64_t batch,
                            const float* scores, int64_t keep, int64_t recent,
                            const int32_t* new_table, int32_t new_max_pages, int32_t* new_lengths,

@@ -41,7 +41,8 @@ def cache():
 @pytest.mark.parametrize("kw,status,msg", [
     ({"dtype": _lib.U8}, 2, "f32, f16 or bf16"), ({"d": 0}, 1, "head_dim"), ({"d": 264}, 1, "head_dim"),
     ({"d": 60}, 1, "16 bytes"), ({"d": 62, "dtype": _lib.F32}, 1, "16 bytes"), ({"page": 0}, 1, "power of two"),
-    ({"page": 24}, 1, "power of two"), ({"kv": 0}, 1, "positive"), ({"pages": 0}, 1, "positive"),
+    ({"page": 24}, 1, "power of two"), ({"kv": 0}, 1, "positive"), ({"kv": 16385}, 1, "16384"), ({"max_pages": (1 << 26) + 1}, 1, "2^30"),
+    ({"pages": (1 << 31) - 1, "kv": 8, "page": 1}, 1, "2^32"), ({"pages": 0}, 1, "positive"),
     ({"pages": 1 << 31}, 1, "2^31"), ({"seqs": 0}, 1, "positive"), ({"max_pages": 1 << 27}, 1, "2^31"),
 ])
 def test_create_refuses(kw, status, msg):
@@ -86,6 +87,7 @@ def rotary(**kw):
     ({"heads": -4}, "heads"), ({"out": None}, "q_out"), ({"k": None}, "null"), ({"seq": None}, "null"),
     ({"slot": None}, "null"), ({"qs": 255}, "strides"), ({"ks": 127}, "strides"), ({"vs": 127}, "strides"),
     ({"out": X}, "overlaps"), ({"out": P((4 << 32) + 2 * (2 * 300 + 255))}, "overlaps"),
+    ({"out": Z}, "overlaps"), ({"v": Y}, "overlaps"), ({"heads": 65536, "qs": 1 << 23}, "heads"),
     ({"rot": {"pairs": 33}}, "pairs"), ({"rot": {"pairs": -1}}, "pairs"), ({"rot": {"cos": None}}, "tables"),
     ({"rot": {"max_pos": 0}}, "tables"), ({"rot": {"axes": 5}}, "axes"), ({"rot": {"axes": 0}}, "axes"),
     ({"rot": {"axis": 1}}, "axis"), ({"rot": {}, "pos": None}, "positions"),
@@ -104,6 +106,8 @@ def test_append_refuses(cache, kw, msg):
     ({"batch": 5}, "sequences"), ({"q": None}, "null"), ({"len": None}, "null"), ({"out": None}, "null"),
     ({"ws": None}, "null"), ({"sc": X}, "only one"), ({"new": X}, "only one"), ({"window": -1}, "window"),
     ({"qs": 255}, "q_stride"), ({"bytes": -1}, "workspace"), ({"ws": P((7 << 32) + 4)}, "workspace"),
+    ({"out": X}, "overlaps"), ({"out": P((4 << 32) + 2 * (3 * 256 - 1))}, "overlaps"),
+    ({"sc": P(8 << 32), "new": P((8 << 32) + 4)}, "overlaps"),
 ])
 def test_attention_refuses(cache, kw, msg):
     lib = _lib.load()
@@ -128,6 +132,7 @@ def test_attention_workspace_holds_the_scores(cache):
     ({"batch": -1}, "sequences"), ({"batch": 5}, "sequences"), ({"keep": 0}, "keep"), ({"keep": 33}, "keep"),
     ({"recent": -1}, "recent"), ({"recent": 9}, "recent"), ({"len": None}, "null"), ({"sc": None}, "null"),
     ({"nt": None}, "null"), ({"nl": None}, "null"), ({"kept": None}, "null"), ({"stride": 7}, "new_score_stride"),
+    ({"new": W}, "two outputs"), ({"nl": P(9 << 32)}, "two outputs"),
     ({"nl": X}, "overlaps"), ({"new": Y}, "overlaps"), ({"kept": TABLE}, "overlaps"), ({"nl": Z}, "overlaps"),
 ])
 def test_evict_refuses(cache, kw, msg):

@@ -2,7 +2,8 @@
 
 The product is the C-ABI library ``libtq4.so`` (include/tq4.h) with hand-written CUDA kernels;
 this package is its Python host side: ``quantized`` mirrors the reference's operator contract
-(``Transmuter.Ops.Quantized.apply/2``) and ``sharded`` the N-sharded multi-GPU path.
+(``Transmuter.Ops.Quantized.apply/2``), ``paged`` serves many sequences over a paged key-value
+cache, and ``sharded`` is the N-sharded multi-GPU path.
 """
 
 from . import _lib  # noqa: F401

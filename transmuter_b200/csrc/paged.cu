@@ -754,8 +754,11 @@ tq4_status tq4_paged_append(const tq4_paged* cache, const void* q, int64_t q_str
     return TQ4_ERR_INVALID_ARGUMENT;
   }
   const int size = dtype_size(d.dtype);
-  if (q && overlaps(q, ((tokens - 1) * q_stride + heads * D) * size, q_out, tokens * heads * D * size)) {
-    set_error("tq4_paged_append: q_out overlaps q");
+  auto bytes = [&](int64_t stride, int64_t n) { return ((tokens - 1) * stride + n * D) * size; };
+  if (q && (overlaps(q, bytes(q_stride, heads), q_out, tokens * heads * D * size) ||
+            overlaps(k, bytes(k_stride, d.kv_heads), q_out, tokens * heads * D * size) ||
+            overlaps(v, bytes(v_stride, d.kv_heads), q_out, tokens * heads * D * size))) {
+    set_error("tq4_paged_append: q_out overlaps q, k or v");
     return TQ4_ERR_INVALID_ARGUMENT;
   }
   AppendArgs a{};
@@ -851,6 +854,12 @@ tq4_status tq4_paged_evict(const tq4_paged* cache, const int32_t* lengths, int64
     for (const auto& i : in)
       if (overlaps(o.p, o.bytes, i.p, i.bytes)) {
         set_error("tq4_paged_evict: an output overlaps an input");
+        return TQ4_ERR_INVALID_ARGUMENT;
+      }
+  for (int i = 0; i < 3; ++i)
+    for (int j = 0; j < i; ++j)
+      if (overlaps(outs[i].p, outs[i].bytes, outs[j].p, outs[j].bytes)) {
+        set_error("tq4_paged_evict: two outputs overlap");
         return TQ4_ERR_INVALID_ARGUMENT;
       }
   a.lengths = lengths;

@@ -1098,6 +1098,16 @@ tq4_status tq4_paged_attention(const tq4_paged* cache, const void* q, int64_t q_
               (long long)q_stride);
     return TQ4_ERR_INVALID_ARGUMENT;
   }
+  const int64_t out_values = batch * heads * d.head_dim, size = dtype_size(d.dtype);
+  if (overlaps(q, ((batch - 1) * q_stride + (int64_t)heads * d.head_dim) * size, out, out_values * size)) {
+    set_error("tq4_paged_attention: out overlaps q");
+    return TQ4_ERR_INVALID_ARGUMENT;
+  }
+  const int64_t score_bytes = batch * d.kv_heads * (int64_t)d.max_pages * d.page_size * 4;
+  if (scores != new_scores && overlaps(scores, score_bytes, new_scores, score_bytes)) {
+    set_error("tq4_paged_attention: new_scores overlaps scores and is not the same buffer");
+    return TQ4_ERR_INVALID_ARGUMENT;
+  }
   const Workspace ws = workspace_of(d, heads, batch, scores != nullptr);
   if (workspace_bytes < ws.bytes || !aligned16(workspace)) {
     set_error("tq4_paged_attention: the workspace must be 16-byte aligned and hold %lld bytes, got %lld",

@@ -150,7 +150,7 @@ class PagedCache:
         sequence ``seq[t]``; seq -1 is padding and nothing of it is touched) and returns their queries,
         both normed and turned by ``rotary`` at ``positions`` (int32 [tokens], or [axes, tokens]).
         q [tokens, heads, head_dim], or None when only the cache is filled; k and v [tokens, kv_heads,
-        head_dim]; views of a merged projection are read in place. ``out`` may not overlap q."""
+        head_dim]; views of a merged projection are read in place. ``out`` may not overlap them."""
         device = self.device
         k, ks = self._rows(k, "k", self.kv_heads)
         v, vs = self._rows(v, "v", self.kv_heads)
