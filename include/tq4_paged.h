@@ -79,7 +79,8 @@ tq4_status tq4_paged_append(const tq4_paged* cache, const void* q, int64_t q_str
                             const int32_t* positions, const tq4_rotary* rotary, void* q_out,
                             void* stream);
 
-/* Bytes of workspace that tq4_paged_attention needs for these sizes on the handle's device. */
+/* Bytes of workspace that tq4_paged_attention needs for these sizes, whatever the lengths and the window (up to 120 MB,
+ * and heads * 4 bytes a slot of the page table's rows with scores; 0 for few short rows without). */
 tq4_status tq4_paged_attention_workspace(const tq4_paged* cache, int heads, int64_t batch,
                                          int with_scores, int64_t* bytes);
 
@@ -93,8 +94,8 @@ tq4_status tq4_paged_attention_workspace(const tq4_paged* cache, int heads, int6
  * may be the same buffer), the softmax weights that eviction goes by are accumulated: slot j of
  * new_scores is that of scores plus the sum over the KV head's query heads of slot j's weight, and
  * slots at and behind lengths[b] are left as they were.
- * workspace: 16-byte aligned device memory that this call has to itself until it has run; what it
- * held before does not matter. Sums, maxima and outputs are accumulated in f32 and in an order that
+ * workspace: 16-byte aligned device memory that this call has to itself until it has run (NULL where
+ * 0 bytes are needed); what it held before does not matter. Sums, maxima and outputs are accumulated in f32 and in an order that
  * depends on the lengths alone: equal calls give equal bits. */
 tq4_status tq4_paged_attention(const tq4_paged* cache, const void* q, int64_t q_stride, int heads,
                                const int32_t* lengths, int64_t batch, float scale, int64_t window,

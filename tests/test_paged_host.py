@@ -104,19 +104,22 @@ def test_append_refuses(cache, kw, msg):
 @pytest.mark.parametrize("kw,msg", [
     ({"heads": 0}, "heads"), ({"heads": 3}, "heads"), ({"heads": 65538}, "heads"), ({"batch": -1}, "sequences"),
     ({"batch": 5}, "sequences"), ({"q": None}, "null"), ({"len": None}, "null"), ({"out": None}, "null"),
-    ({"ws": None}, "null"), ({"sc": X}, "only one"), ({"new": X}, "only one"), ({"window": -1}, "window"),
+    ({"ws": None}, "workspace"), ({"sc": X}, "only one"), ({"new": X}, "only one"), ({"window": -1}, "window"),
     ({"qs": 255}, "q_stride"), ({"bytes": -1}, "workspace"), ({"ws": P((7 << 32) + 4)}, "workspace"),
     ({"out": X}, "overlaps"), ({"out": P((4 << 32) + 2 * (3 * 256 - 1))}, "overlaps"),
     ({"sc": P(8 << 32), "new": P((8 << 32) + 4)}, "overlaps"),
 ])
-def test_attention_refuses(cache, kw, msg):
+def test_attention_refuses(kw, msg):
     lib = _lib.load()
+    st, cache = create(desc(max_pages=5000))  # room for long sequences: a workspace is needed
+    assert st == 0
     n = ctypes.c_int64()
     assert lib.tq4_paged_attention_workspace(cache, 4, 3, 0, ctypes.byref(n)) == 0 and n.value > 0
     st = lib.tq4_paged_attention(
         cache, kw.get("q", X), kw.get("qs", 256), kw.get("heads", 4), kw.get("len", Z), kw.get("batch", 3), 0.125,
         kw.get("window", 0), kw.get("sc"), kw.get("new"), kw.get("out", Y), kw.get("ws", W), n.value + kw.get("bytes", 0), None)
     assert st == 1 and msg in _lib.last_error()
+    lib.tq4_paged_destroy(cache)
 
 
 def test_attention_workspace_holds_the_scores(cache):
@@ -124,7 +127,12 @@ def test_attention_workspace_holds_the_scores(cache):
     a, b = ctypes.c_int64(), ctypes.c_int64()
     lib.tq4_paged_attention_workspace(cache, 4, 3, 0, ctypes.byref(a))
     lib.tq4_paged_attention_workspace(cache, 4, 3, 1, ctypes.byref(b))
-    assert b.value >= a.value + 3 * 4 * 5 * 16 * 4
+    assert a.value == 0 and b.value == 3 * 4 * 5 * 16 * 4  # few short rows: nothing but the scores
+    st, wide = create(desc(max_pages=5000))
+    lib.tq4_paged_attention_workspace(wide, 4, 3, 0, ctypes.byref(a))
+    lib.tq4_paged_attention_workspace(wide, 4, 3, 1, ctypes.byref(b))
+    assert a.value > 0 and b.value >= a.value + 3 * 4 * 5000 * 16 * 4
+    lib.tq4_paged_destroy(wide)
     assert lib.tq4_paged_attention_workspace(cache, 4, 3, 1, None) == 1
 
 

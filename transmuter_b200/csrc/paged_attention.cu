@@ -938,15 +938,35 @@ Shape shape_of(const tq4_paged_desc& d, int heads, int64_t batch) {
   return s;
 }
 
-// Offsets of the workspace's parts, in bytes, each a multiple of 16.
+// CTAs of a row for the cluster kernel; 0 where the line's kernels are to be used. The cluster kernel takes rows
+// that do not fill the SMs twice over, with room in the page table (or the window) for few units a warp, and with
+// all heads of a KV head in one row where there are scores.
+int cluster_size(const tq4_paged_desc& d, const Shape& s, int64_t batch, int64_t window, bool with_scores) {
+  const int64_t rows = batch * d.kv_heads * s.tiles;
+  int64_t slots = (int64_t)d.max_pages * d.page_size;
+  if (window > 0) slots = std::min(slots, window + s.unit);
+  const int64_t units = (slots + s.unit - 1) / s.unit;
+  if (rows > s.ctas || (with_scores && s.tiles > 1)) return 0;
+  int c = 1;
+  while (c < kMaxClusterCtas && rows * c * 2 <= s.ctas && units > (int64_t)c * s.warps) c *= 2;
+  return units <= (int64_t)c * s.warps * kClusterUnits ? c : 0;
+}
+
+// Offsets of the workspace's parts, in bytes, each a multiple of 16. What the cluster kernel takes whatever the
+// window needs none but the scores'.
 struct Workspace {
   int64_t seq_first, ends, joins, stats, ml, parts, weights, bytes;
 };
 Workspace workspace_of(const tq4_paged_desc& d, int heads, int64_t batch, bool with_scores) {
   auto up = [](int64_t n) { return (n + 15) / 16 * 16; };
   const Shape s = shape_of(d, heads, batch);
+  const bool line = cluster_size(d, s, batch, 0, with_scores) == 0;
   const int64_t slots = s.grid * s.warps * 2 * s.tile;
-  Workspace w;
+  Workspace w{};
+  if (!line) {
+    w.bytes = with_scores ? up(batch * heads * (int64_t)d.max_pages * d.page_size * 4) : 0;
+    return w;
+  }
   w.seq_first = up(sizeof(Plan));
   w.ends = w.seq_first + up(batch * 8);
   w.joins = w.ends + up(s.grid * s.warps);
@@ -973,20 +993,6 @@ tq4_status check_attention(const tq4_paged* cache, int heads, int64_t batch) {
     return TQ4_ERR_INVALID_ARGUMENT;
   }
   return TQ4_OK;
-}
-
-// CTAs of a row for the cluster kernel; 0 where the line's kernels are to be used: rows that do not fill the SMs
-// twice over, with room in the page table for few units a warp, and all heads of a KV head in one row where
-// there are scores.
-int cluster_size(const AttnArgs& a) {
-  const int64_t rows = a.batch * a.cache.kv_heads * a.tiles;
-  int64_t slots = a.cache.max_slots;
-  if (a.window > 0) slots = std::min(slots, a.window + a.unit);
-  const int64_t units = (slots + a.unit - 1) / a.unit;
-  if (rows > a.ctas || (a.new_scores && a.tiles > 1)) return 0;
-  int c = 1;
-  while (c < kMaxClusterCtas && rows * c * 2 <= a.ctas && units > (int64_t)c * a.warps) c *= 2;
-  return units <= (int64_t)c * a.warps * kClusterUnits ? c : 0;
 }
 
 template <typename T, int DT, int TILE>
@@ -1089,8 +1095,8 @@ tq4_status tq4_paged_attention(const tq4_paged* cache, const void* q, int64_t q_
   TQ4_TRY(check_attention(cache, heads, batch));
   const tq4_paged_desc& d = cache->desc;
   if (batch == 0) return TQ4_OK;
-  if (!q || !lengths || !out || !workspace || (scores != nullptr) != (new_scores != nullptr)) {
-    set_error("tq4_paged_attention: null q, lengths, out or workspace, or only one of scores and new_scores");
+  if (!q || !lengths || !out || (scores != nullptr) != (new_scores != nullptr)) {
+    set_error("tq4_paged_attention: null q, lengths or out, or only one of scores and new_scores");
     return TQ4_ERR_INVALID_ARGUMENT;
   }
   if (window < 0 || q_stride < (int64_t)heads * d.head_dim) {
@@ -1109,7 +1115,7 @@ tq4_status tq4_paged_attention(const tq4_paged* cache, const void* q, int64_t q_
     return TQ4_ERR_INVALID_ARGUMENT;
   }
   const Workspace ws = workspace_of(d, heads, batch, scores != nullptr);
-  if (workspace_bytes < ws.bytes || !aligned16(workspace)) {
+  if (workspace_bytes < ws.bytes || !aligned16(workspace) || (ws.bytes > 0 && !workspace)) {
     set_error("tq4_paged_attention: the workspace must be 16-byte aligned and hold %lld bytes, got %lld",
               (long long)ws.bytes, (long long)workspace_bytes);
     return TQ4_ERR_INVALID_ARGUMENT;
@@ -1148,7 +1154,7 @@ tq4_status tq4_paged_attention(const tq4_paged* cache, const void* q, int64_t q_
   a.pieces = (int)shape.grid * shape.warps;
   a.parts = reinterpret_cast<float*>(w + ws.parts);
   a.weights = reinterpret_cast<float*>(w + ws.weights);
-  a.cluster = cluster_size(a);
+  a.cluster = cluster_size(d, shape, batch, window, scores != nullptr);
   if (batch * d.kv_heads * a.tiles > ((int64_t)1 << 30)) {
     set_error("tq4_paged_attention: more than 2^30 rows of sequences and KV heads");
     return TQ4_ERR_INVALID_ARGUMENT;

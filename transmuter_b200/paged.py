@@ -131,19 +131,21 @@ class PagedCache:
             pass
 
     def _rows(self, x, name, heads):
-        """x [tokens, heads, head_dim] with each token's heads contiguous, copied where they are not, and the
-        distance of its tokens."""
-        if not (isinstance(x, torch.Tensor) and x.dtype is self.dtype and x.device == self.device and x.dim() == 3
-                and x.shape[2] == self.head_dim and x.shape[1] == (heads or x.shape[1])):
+        """x [tokens, heads, head_dim] with each token's heads contiguous, copied where they are not; the
+        distance of its tokens, and tokens and heads."""
+        shape = x.shape if isinstance(x, torch.Tensor) else ()
+        if len(shape) != 3 or not (x.dtype is self.dtype and shape[2] == self.head_dim and heads in (None, shape[1])
+                                   and x.device == self.device):
             raise ArgumentError(f"paged cache: {name} must be {self.dtype} [tokens, {heads or 'heads'}, {self.head_dim}] "
                                 f"on {self.device}")
-        width = x.shape[1] * self.head_dim
+        tokens, heads, d = shape
+        width = heads * d
         if not x.is_contiguous():
-            s = x.stride()
-            if s[2] == 1 and (s[1] == self.head_dim or x.shape[1] == 1) and (s[0] >= width or x.shape[0] <= 1):
-                return x, max(s[0], width)
+            s0, s1, s2 = x.stride()
+            if s2 == 1 and (s1 == d or heads == 1) and (s0 >= width or tokens <= 1):
+                return x, max(s0, width), tokens, heads
             x = x.contiguous()
-        return x, width
+        return x, width, tokens, heads
 
     def append(self, q, k, v, seq, slot, positions=None, rotary=None, out=None):
         """Writes the keys and values of new tokens into the cache (token t is slot ``slot[t]`` of
@@ -152,22 +154,22 @@ class PagedCache:
         q [tokens, heads, head_dim], or None when only the cache is filled; k and v [tokens, kv_heads,
         head_dim]; views of a merged projection are read in place. ``out`` may not overlap them."""
         device = self.device
-        k, ks = self._rows(k, "k", self.kv_heads)
-        v, vs = self._rows(v, "v", self.kv_heads)
-        tokens = k.shape[0]
-        if v.shape[0] != tokens:
-            raise ArgumentError(f"paged cache: {v.shape[0]} values for {tokens} keys")
+        k, ks, tokens, _ = self._rows(k, "k", self.kv_heads)
+        v, vs, values, _ = self._rows(v, "v", self.kv_heads)
+        if values != tokens:
+            raise ArgumentError(f"paged cache: {values} values for {tokens} keys")
         heads = qs = 0
         q_p = out_p = pos_p = ref = None
         if q is not None:
-            q, qs = self._rows(q, "q", None)
-            heads = q.shape[1]
-            if q.shape[0] != tokens or heads == 0:
-                raise ArgumentError(f"paged cache: {q.shape[0]} queries of {heads} heads for {tokens} keys")
+            q, qs, queries, heads = self._rows(q, "q", None)
+            if queries != tokens or heads == 0:
+                raise ArgumentError(f"paged cache: {queries} queries of {heads} heads for {tokens} keys")
             q_p = q.data_ptr()
             if out is None:
                 out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            out_p = _pointer(out, "out", q.shape, self.dtype, device)
+                out_p = out.data_ptr()
+            else:
+                out_p = _pointer(out, "out", q.shape, self.dtype, device)
         elif out is not None:
             raise ArgumentError("paged cache: out without q")
         seq_p = _pointer(seq, "seq", (tokens,), torch.int32, device)
@@ -190,8 +192,7 @@ class PagedCache:
         (f32 [batch, kv_heads, max_pages * page_size]) each slot's softmax weights, summed over the
         query heads of a KV head, are added to them: in place, or into ``new_scores``."""
         device = self.device
-        q, qs = self._rows(q, "q", None)
-        batch, heads, _ = q.shape
+        q, qs, batch, heads = self._rows(q, "q", None)
         if heads == 0 or heads % self.kv_heads:
             raise ArgumentError(f"paged cache: {heads} query heads are not a multiple of {self.kv_heads} KV heads")
         if batch > self.max_seqs:
@@ -206,7 +207,9 @@ class PagedCache:
             raise ArgumentError("paged cache: new_scores without scores")
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        out_p = _pointer(out, "out", q.shape, self.dtype, device)
+            out_p = out.data_ptr()
+        else:
+            out_p = _pointer(out, "out", q.shape, self.dtype, device)
         key = (heads, batch, scores is not None)
         nbytes = self._workspace.get(key)
         if nbytes is None:
@@ -215,10 +218,10 @@ class PagedCache:
             nbytes = self._workspace[key] = n.value
         # a workspace of its own for each call, from torch's allocator: calls on several streams and
         # captured graphs never share one
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         _lib.check(self._lib.tq4_paged_attention(
             self._handle, q.data_ptr(), qs, heads, len_p, batch, self._scale if scale is None else scale, window, in_p, new_p,
-            out_p, ws.data_ptr(), nbytes, _raw_stream(self._index)))
+            out_p, ws.data_ptr() if nbytes else None, nbytes, _raw_stream(self._index)))
         return out
 
     def evict(self, lengths, scores, keep, recent, new_table, new_scores=None):
