@@ -572,9 +572,9 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
 
 namespace {
 
-// Rows of up to this many bytes of K and V are moved by the selection's own CTAs: a launch less (26 -> 11 us for one
-// short sequence, with the selection's other steps), but only as many SMs as it has CTAs.
-constexpr int64_t kMoveInSelection = 4 << 20;
+// Up to this many bytes of K and V a CTA, the rows are moved by the selection's own CTAs: a launch less, but only as
+// many SMs as it has CTAs (3 rows of 1 MB each took 42 us that way, 7.5 us by a kernel of its own).
+constexpr int64_t kMoveInSelection = 160 << 10;
 
 // Whether the rows come in chunks of VE values (*taken), and the launch if so.
 template <typename T, int VE>
@@ -648,8 +648,7 @@ tq4_status launch_evict(EvictArgs& a, int64_t rows, cudaStream_t st) {
   const int64_t share = (slots + cluster - 1) / cluster;
   a.key_room = (int)std::min<int64_t>(share, 40 * 1024);
   const unsigned y = (unsigned)std::min<int64_t>(rows, 65535), z = (unsigned)((rows + y - 1) / y);
-  const int64_t bytes = rows * a.keep * a.row_bytes * 2;
-  a.move = bytes <= kMoveInSelection;
+  a.move = (int64_t)a.keep * a.row_bytes * 2 <= cluster * kMoveInSelection;
   const bool small = share <= 2048;
   const size_t smem = (size_t)a.key_room * 4;
   if (small) TQ4_TRY(launch_select<256>(a, dim3(cluster, y, z), smem, st));

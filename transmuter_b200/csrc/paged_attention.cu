@@ -204,12 +204,12 @@ template <typename T, int DT, int TILE> constexpr int part_smem(int head_dim) {
 }
 
 // Sends for a unit of KV head kvh, its keys and behind them its values, from slot p0 on. `page` is where lane i's
-// slot lies, or all of them (WHOLE). *valid gets a bit for each slot that counts; rows of others may hold
-// anything, NaN too, and become zeros.
+// slot lies (look_up_page). *valid gets a bit for each slot that counts; rows of others may hold anything, NaN too, and become
+// zeros.
 //
-// WHOLE: head_dim is DT and a page holds whole units. Then a unit's keys are one run of memory, as are its
-// values: one page lookup and constant offsets instead of one row address for each chunk (the loads of
-// a unit take 30 instructions a lane instead of 300).
+// WHOLE: head_dim is DT, so that a lane's chunks lie in rows and columns known to the compiler. Where a page holds
+// whole units too, a unit's keys are one run of memory, as are its values, and all offsets are constants (the loads
+// of a unit then take 30 instructions a lane instead of 300).
 template <typename T, int DT, int U, bool WHOLE>
 __device__ __forceinline__ void load_rows(const AttnArgs& a, char* slot, uint32_t* valid, Span span, int p0, int kvh, int page) {
   constexpr int VN = 16 / sizeof(T);
@@ -226,10 +226,23 @@ __device__ __forceinline__ void load_rows(const AttnArgs& a, char* slot, uint32_
   const int in_page = (1 << c.page_log2) - 1;
   if constexpr (WHOLE) {
     constexpr int C = DT / VN, PITCH = row_chunks<T>(DT) * 16;
+    const uint32_t to = dst + (lane / C) * PITCH + (lane % C) * 16;
+    if ((1 << c.page_log2) < U) {  // smaller pages: a lane's rows by shuffle
+      const uint32_t row = first + (p & in_page);
+#pragma unroll
+      for (int j = 0; j < U * C / 32; ++j) {
+        const int at_row = j * 32 / C * PITCH + j * 32 % C * 16, from = lane / C + j * 32 / C;
+        const uint32_t rw = __shfl_sync(0xffffffffu, row, from);
+        const bool take = (mask >> from) & 1;
+        const int64_t off = take ? (int64_t)rw * (DT * (int)sizeof(T)) + (lane % C) * 16 + j * 32 % C * 16 : 0;
+        cp_async16(to + at_row, static_cast<const char*>(a.k_pages) + off, take);
+        cp_async16(to + U * PITCH + at_row, static_cast<const char*>(a.v_pages) + off, take);
+      }
+      return;
+    }
     const int64_t off = (int64_t)(first + (p0 & in_page)) * (DT * (int)sizeof(T)) + lane * 16;
     const char* kp = static_cast<const char*>(a.k_pages) + off;
     const char* vp = static_cast<const char*>(a.v_pages) + off;
-    const uint32_t to = dst + (lane / C) * PITCH + (lane % C) * 16;
     if (mask == (U == 32 ? 0xffffffffu : (1u << (U & 31)) - 1)) {
 #pragma unroll
       for (int j = 0; j < U * C / 32; ++j) {
@@ -292,11 +305,13 @@ __device__ __forceinline__ void load_rows(const AttnArgs& a, char* slot, uint32_
     }
   }
 }
-// The page of the unit's slot p0 + lane, or of p0 (WHOLE); -1 outside the span.
+// The page of the unit's slot p0 + lane, -1 outside the span; where a page holds whole units and rows are WHOLE
+// (load_rows), the unit's page in every lane.
 template <int U, bool WHOLE>
 __device__ __forceinline__ int look_up_page(const AttnArgs& a, int b, Span span, int p0) {
-  const int lane = threadIdx.x & 31, p = p0 + (WHOLE ? 0 : lane);
-  if (WHOLE || (lane < U && p >= span.lo && p < span.hi))
+  const bool one = WHOLE && (1 << a.cache.page_log2) >= U;
+  const int lane = threadIdx.x & 31, p = one ? p0 : p0 + lane;
+  if (one || (lane < U && p >= span.lo && p < span.hi))
     return a.cache.table[(int64_t)b * a.cache.max_pages + (p >> a.cache.page_log2)];
   return -1;
 }
@@ -419,7 +434,7 @@ __global__ void __launch_bounds__(kWarpsOf<T, TILE> * 32, DT <= 128 ? 2 : 1)
   };
 
   // ---- this warp's loads ----
-  // A unit's page is looked up one unit ahead of its use: by lane i for slot i, or for all of them.
+  // A unit's pages are looked up one unit ahead of their use.
   Piece cur = {find_chunk(a, line, blockIdx.x), warp};  // being folded
   Piece coming = cur;                                   // being loaded
   if (warp == 0) draw();
@@ -997,7 +1012,7 @@ tq4_status check_attention(const tq4_paged* cache, int heads, int64_t batch) {
 
 template <typename T, int DT, int TILE>
 tq4_status launch_cluster(const AttnArgs& a, int c, cudaStream_t st) {
-  const bool whole = a.cache.head_dim == DT && (1 << a.cache.page_log2) >= a.unit;
+  const bool whole = a.cache.head_dim == DT;
   const auto kern = whole ? attention_cluster_kernel<T, DT, TILE, true> : attention_cluster_kernel<T, DT, TILE, false>;
   static std::atomic<uint64_t> set[2];  // per device, per instantiation
   TQ4_CUDA(set_smem_limit_once(kern, part_smem<T, DT, TILE>(DT), set[whole]));
@@ -1026,7 +1041,7 @@ tq4_status launch_part(AttnArgs& a, int64_t grid, cudaStream_t st) {
     return TQ4_ERR_UNSUPPORTED;
   }
   if (a.cluster) return launch_cluster<T, DT, TILE>(a, a.cluster, st);
-  const bool whole = a.cache.head_dim == DT && (1 << a.cache.page_log2) >= a.unit;
+  const bool whole = a.cache.head_dim == DT;
   const auto kern = whole ? attention_part_kernel<T, DT, TILE, true> : attention_part_kernel<T, DT, TILE, false>;
   static std::atomic<uint64_t> set[2];  // per device, per instantiation
   TQ4_CUDA(set_smem_limit_once(kern, part_smem<T, DT, TILE>(DT), set[whole]));
