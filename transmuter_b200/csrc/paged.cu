@@ -359,7 +359,7 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int64_t b, int h, 
 }
 
 constexpr int kBins = 2048;     // of a pass over 11 bits of the keys
-constexpr int kMaxCluster = 8;  // CTAs of a row
+constexpr int kMaxCluster = 8;  // CTAs of a row (of 131072 slots: 16 take 89 us, 8 take 42 us, 4 about 39 us)
 
 // One cluster per (sequence, KV head): which slots are kept. A CTA has a share of the candidates, in shared memory
 // as keys. The smallest kept key is found by radix selection in three passes of 11, 11 and 10 bits: the
