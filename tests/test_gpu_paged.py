@@ -665,3 +665,47 @@ def test_served_batch_prompts_steps_and_eviction(dtype):
         check_attention(out, scores, c, qo, lengths, 0, old)
         # each sequence's weights of a step add up to one a query head
         assert torch.allclose((scores - old).sum(-1), torch.full((3, kv), float(heads // kv), device=DEV), atol=1e-4)
+
+
+# ---- the workspace ------------------------------------------------------------------------------
+
+def attention_in(c, q, lengths, ws, scores=None, new=None, window=0):
+    """The C entry with a workspace of the caller's and an output between guards: (output, whether the guards held)."""
+    import ctypes
+    batch, heads, d = q.shape
+    n = ctypes.c_int64()
+    _lib.check(c._lib.tq4_paged_attention_workspace(c._handle, heads, batch, int(scores is not None), ctypes.byref(n)))
+    assert ws.numel() >= n.value
+    guard = 1 << 14
+    room = torch.full((q.numel() + 2 * guard,), 3.0, device=DEV, dtype=q.dtype)
+    out = room[guard:-guard].view(q.shape)
+    _lib.check(c._lib.tq4_paged_attention(
+        c._handle, q.data_ptr(), heads * d, heads, lengths.data_ptr(), batch, 1 / math.sqrt(d), window,
+        scores.data_ptr() if scores is not None else None, new.data_ptr() if new is not None else None, out.data_ptr(),
+        ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream))
+    return out, bool((room[:guard] == 3).all() and (room[-guard:] == 3).all())
+
+
+# what a workspace may hold before a call: zeros, ones, the largest and all bits set
+FILLS = [0, 1, 0x7F, 0xFF]
+
+
+@pytest.mark.parametrize("dtype,heads,kv,lengths", [
+    (BF16, 8, 2, [3000, 0, 900, 1, 5000]), (F32, 16, 2, [700, 2, 1500]), (F16, 40, 2, [20000]), (BF16, 4, 4, [0, 0]),
+    (F32, 6, 2, [(i * 37) % 90 for i in range(400)]),
+], ids=lambda x: str(x)[:40])
+def test_attention_reads_nothing_that_an_earlier_call_left(dtype, heads, kv, lengths):
+    k, v, table, _ = make_pool(lengths, kv, 16, 64, dtype, 21, width=width_of(True, lengths, 16))
+    c = paged.PagedCache(k, v, table)
+    q = torch.randn(len(lengths), heads, 64, device=DEV).to(dtype)
+    old = torch.rand(len(lengths), kv, c.max_slots, device=DEV)
+    n = ints(lengths)
+    new = torch.zeros_like(old)
+    want, want_s = c.attention(q, n), c.attention(q, n, scores=old, new_scores=new)
+    most = torch.empty(c._workspace[(heads, len(lengths), True)], dtype=torch.uint8, device=DEV)
+    for fill in FILLS:
+        out, held = attention_in(c, q, n, most.fill_(fill))
+        assert held and torch.equal(out, want)
+        got = torch.zeros_like(old)
+        out, held = attention_in(c, q, n, most.fill_(fill), old, got)
+        assert held and torch.equal(out, want_s) and torch.equal(got, new)

@@ -369,12 +369,17 @@ __global__ void __launch_bounds__(kWarpsOf<T, TILE> * 32, DT <= 128 ? 2 : 1)
   pdl_trigger();
   make_line(a, line, red);
   const int n_chunks = line.plan.ctas * line.plan.levels;
-  if (blockIdx.x == 0) {
+  // The second kernel needs the plan, and for the scores where each sequence begins. Every CTA that begins and has a
+  // chunk writes them, all the same values: any one of them, the first too, may be taken by another before it begins,
+  // but whoever takes one has begun and has a chunk itself. (Where there is no chunk, none is taken.)
+  if ((int)blockIdx.x < n_chunks || blockIdx.x == 0) {
     if (tid == 0) *a.plan = line.plan;
-    int64_t at = tid ? line.ends[tid - 1] : 0;
-    for (int b = tid * line.per; b < (tid + 1) * line.per && b < a.batch; ++b) {
-      a.seq_first[b] = at;
-      at += (int64_t)units_of(a, span_of(a, b)) * rows;
+    if (a.new_scores) {
+      int64_t at = tid ? line.ends[tid - 1] : 0;
+      for (int b = tid * line.per; b < (tid + 1) * line.per && b < a.batch; ++b) {
+        a.seq_first[b] = at;
+        at += (int64_t)units_of(a, span_of(a, b)) * rows;
+      }
     }
   }
   if ((int)blockIdx.x >= n_chunks) return;  // the grid was made for longer sequences

@@ -52,7 +52,7 @@ struct AttnArgs {
   float* new_scores;
   // workspace
   Plan* plan;
-  int64_t* seq_first;  // [batch]: the line's place where a sequence begins
+  int64_t* seq_first;  // [batch]: the line's place where a sequence begins; written and read where there are scores
   uint8_t* ends;       // [grid * warps], by piece: 1 where a row ends that began in an earlier one
   int4* joins;         // [grid * warps]: that row: sequence, row, the piece it began in
   float* stats;    // [batch][heads][2]: m, 1 / l of rows that lie in one piece
