@@ -178,7 +178,9 @@ tq4_status tq4_device_status(int device, int32_t* code);
  * decoder kernels; the peer-flag waits of N-sharded calls), in SM clock cycles: 0 restores the
  * default of 2e9 (about one second at the B200's clocks), other values must be at least 1000.
  * Synchronizes the device first. Meant for failure tests and for watchdogs that must fire
- * sooner; a limit below a healthy call's own waits makes that call report a timeout. */
+ * sooner; a limit below a healthy call's own waits makes that call report a timeout and leave its
+ * outputs unfinished. (Before a kernel that gave up ends, it still waits for its own copies under way, up to the
+ * default limit.) */
 tq4_status tq4_set_wait_limit(int device, int64_t cycles);
 
 /* Runs the peer-flag wait of the N-sharded kernels on `stream` against a flag that nothing ever

@@ -59,10 +59,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   return true;
 }
 
-// Waits (bounded) for a phase that is known to complete; used when winding down.
+// Waits (bounded) for a phase that is known to complete; used when winding down. Not by the device's wait limit: what is
+// still under way is written into the CTA's shared memory, which goes to another CTA once this one leaves, so a limit that
+// was set shorter than a healthy copy must not end this wait.
+constexpr long long kDrainCycles = 2000000000LL;  // about a second, the default wait limit
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
-  const long long t0 = clock64(), limit = wait_limit();
-  while (!mbar_test(bar, parity) && clock64() - t0 < limit) {
+  const long long t0 = clock64();
+  while (!mbar_test(bar, parity) && clock64() - t0 < kDrainCycles) {
   }
 }
 
