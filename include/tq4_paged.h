@@ -13,7 +13,8 @@
  * Pointers are device pointers of the handle's device unless "host" is said; every call enqueues
  * on `stream` and may be captured into a CUDA graph (lengths, slots and tables live on the device).
  * A length, slot, sequence, position or page number out of range never leads out of bounds: what it
- * stands for is skipped and the device status set to 0x200 (tq4_device_status).
+ * stands for is skipped and the device status set to 0x200 (tq4_device_status). Where the attention's own waits ran
+ * out (0x107, tq4_set_wait_limit), what the call's outputs hold is not defined.
  */
 #ifndef TQ4_PAGED_H
 #define TQ4_PAGED_H

@@ -709,3 +709,52 @@ def test_attention_reads_nothing_that_an_earlier_call_left(dtype, heads, kv, len
         got = torch.zeros_like(old)
         out, held = attention_in(c, q, n, most.fill_(fill), old, got)
         assert held and torch.equal(out, want_s) and torch.equal(got, new)
+
+
+ATTENTION_TIMEOUT = 0x107
+
+
+@pytest.mark.parametrize("dtype,heads,kv,count,most", [
+    (BF16, 8, 2, 20000, 70), (F32, 8, 1, 20000, 40), (F16, 32, 2, 60, 9000), (F32, 4, 2, 3, 9000),
+], ids=str)
+def test_attention_of_which_a_wait_runs_out(dtype, heads, kv, count, most):
+    """With the shortest wait limit, warps give up waiting for their next chunk (a chunk among 20000 sequences takes longer
+    to find than that): the call says so or is right, writes nothing outside its outputs whatever the workspace held, and
+    the next call is as ever."""
+    ps, d, pages = 16, 64, 600
+    g = torch.Generator(DEV).manual_seed(31)
+    k, v = (torch.randn(pages, kv, ps, d, device=DEV, generator=g).to(dtype) for _ in range(2))
+    table = torch.randint(0, pages, (count, -(-most // ps)), device=DEV, generator=g, dtype=torch.int32)  # pages are shared
+    c = paged.PagedCache(k, v, table)
+    q = torch.randn(count, heads, d, device=DEV, generator=g).to(dtype)
+    n = torch.randint(0, most + 1, (count,), device=DEV, generator=g, dtype=torch.int32)
+    old = torch.rand(count, kv, c.max_slots, device=DEV, generator=g)
+    new = torch.zeros_like(old)
+    want, want_s = c.attention(q, n), c.attention(q, n, scores=old, new_scores=new)
+    ws = torch.empty(c._workspace[(heads, count, True)], dtype=torch.uint8, device=DEV)
+    small = ws.view(torch.int32)[:ws.numel() // 4]
+    codes = []
+    for fill in FILLS + [None]:
+        for scores in (False, True):
+            if fill is None:
+                small.fill_(1)  # numbers that could be a row's
+            else:
+                ws.fill_(fill)
+            got = torch.zeros_like(old) if scores else None
+            torch.cuda.synchronize()
+            _lib.check(_lib.load().tq4_set_wait_limit(0, 1000))
+            try:
+                out, held = attention_in(c, q, n, ws, old if scores else None, got)
+                torch.cuda.synchronize()
+                codes.append(device_status())
+            finally:
+                _lib.check(_lib.load().tq4_set_wait_limit(0, 0))
+            assert held and codes[-1] in (0, ATTENTION_TIMEOUT)
+            if scores:
+                behind = torch.arange(c.max_slots, device=DEV) >= n[:, None, None]
+                assert not got[behind.expand_as(got)].any()
+            if codes[-1] == 0:
+                assert torch.equal(out, want_s if scores else want)
+            assert torch.equal(c.attention(q, n), want)  # the default limit is back
+    print(codes)
+    assert count < 20000 or ATTENTION_TIMEOUT in codes

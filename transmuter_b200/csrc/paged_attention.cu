@@ -760,7 +760,10 @@ __device__ __forceinline__ void join_head(const AttnArgs& a, int last, int g, in
   const int D = a.cache.head_dim, tid = threadIdx.x;
   const int4 row = a.joins[last];
   const int kvh = row.y / a.tiles, g0 = (row.y - kvh * a.tiles) * a.tile, first = row.z;
-  if (g >= a.group - g0) return;  // the same for the block
+  // All the same for the block. Pieces of a chunk that nobody did, since a wait ran out, hold whatever the workspace
+  // held before the call: nothing is read or written by what cannot be a row.
+  if (row.x < 0 || row.x >= a.batch || row.y < 0 || row.y >= a.cache.kv_heads * a.tiles || first < 0 || first > last) return;
+  if (g >= a.group - g0) return;
   const int lanes = kFinishThreads / cols, j = tid / cols, col = tid - j * cols, d = (col0 + col) * 4;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   float2 ml = make_float2(-INFINITY, 0.f);
