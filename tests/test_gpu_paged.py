@@ -758,3 +758,74 @@ def test_attention_of_which_a_wait_runs_out(dtype, heads, kv, count, most):
             assert torch.equal(c.attention(q, n), want)  # the default limit is back
     print(codes)
     assert count < 20000 or ATTENTION_TIMEOUT in codes
+
+
+# ---- values that are not finite -----------------------------------------------------------------
+
+def bits(x):
+    return x.contiguous().view(torch.int32 if x.dtype == F32 else torch.int16)
+
+
+def append_into(c, q, k, v, rot=None, pos=None):
+    """One append of q, k, v [tokens, heads, d] to the first slots of sequence 0: (queries, keys, values) as they then stand."""
+    n = q.shape[0]
+    out = c.append(q, k, v, ints([0] * n), ints(range(n)), pos, rot)
+    at = [(c.page_table[0, j // c.page_size].item(), j % c.page_size) for j in range(n)]
+    return out, torch.stack([c.k_pages[p, :, r] for p, r in at]), torch.stack([c.v_pages[p, :, r] for p, r in at])
+
+
+# dtype, d, pairs, interleaved, offset of the views
+UNTURNED = [
+    (BF16, 128, 32, False, 0), (BF16, 128, 32, True, 0), (F16, 128, 0, False, 0), (F32, 64, 16, False, 0), (F32, 64, 16, True, 0),
+    (F16, 72, 18, False, 0), (BF16, 72, 9, True, 0), (F16, 128, 32, False, 2), (BF16, 128, 32, True, 1), (F32, 256, 5, False, 0),
+]
+
+
+def special_rows(n, heads, d, dtype, offset, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, heads * d + offset, generator=g)
+    for i, value in enumerate([math.inf, -math.inf, math.nan, -0.0, 1e-45, math.inf]):
+        x[:, offset + i * 7 + 3::53] = value
+    return x.to(DEV, dtype)[:, offset:].unflatten(1, (heads, d))
+
+
+@pytest.mark.parametrize("case", UNTURNED, ids=str)
+def test_append_copies_what_is_not_turned(case):
+    """Without a norm, values that no pair turns come out bit for bit, whatever stands beside them: infinities, NaN, -0."""
+    dtype, d, pairs, interleaved, offset = case
+    c = simple_cache(dtype, lengths=(12, 1), kv=2, ps=4, d=d)
+    q, k, v = (special_rows(9, h, d, dtype, offset, i) for i, h in enumerate((5, 2, 2)))
+    ang = torch.randn(9, pairs, device=DEV)
+    rot = paged.Rotary(ang.cos(), ang.sin(), interleaved=interleaved)
+    for r, rest in ((rot, 2 * pairs), (None, 0)):
+        for x, y in zip((q, k, v), append_into(c, q, k, v, r, ints(range(9)) if r else None)):
+            assert torch.equal(bits(x[..., d if x is v else rest:]), bits(y[..., d if x is v else rest:]))
+        assert torch.equal(bits(v), bits(y))
+
+
+@pytest.mark.parametrize("case", UNTURNED, ids=str)
+def test_append_keeps_an_infinity_in_its_pair(case):
+    """An infinite value of a head changes its own output and its partner's, with or without a norm of zero angles; with a norm
+    it makes the head's finite values 0."""
+    dtype, d, pairs, interleaved, offset = case
+    c = simple_cache(dtype, lengths=(12, 1), kv=2, ps=4, d=d)
+    g = torch.Generator().manual_seed(5)
+    clean = [torch.randn(8, h * d + offset, generator=g).to(DEV, dtype) for h in (5, 2, 2)]
+    ang = torch.randn(8, pairs, device=DEV)
+    w = torch.rand(d, device=DEV) + 0.5
+    pos = ints(range(8))
+    for i in sorted({0, 1, pairs, 2 * pairs, 2 * pairs + 1, d // 2, d - 1} & set(range(d))):
+        other = i if i >= 2 * pairs else i ^ 1 if interleaved else (i + pairs) % (2 * pairs)
+        hot = [x.clone() for x in clean]
+        for x in hot[:2]:
+            x[:, offset + i::d] = math.inf
+        view = lambda x: x[:, offset:].unflatten(1, (-1, d))
+        rot = paged.Rotary(ang.cos(), ang.sin(), interleaved=interleaved)
+        want, got = ([y.clone() for y in append_into(c, *map(view, x), rot, pos)] for x in (clean, hot))
+        for x, y in zip(want, got):
+            rest = [e for e in range(d) if e not in (i, other)]
+            assert torch.equal(bits(x[..., rest]), bits(y[..., rest]))
+        rot = paged.Rotary(ang.cos(), ang.sin(), interleaved=interleaved, q_weight=w, k_weight=w)
+        for y in append_into(c, *map(view, hot), rot, pos)[:2]:
+            rest = [e for e in range(d) if e not in (i, other)]
+            assert not y[..., rest].any() and y[..., i].isnan().all()

@@ -72,7 +72,10 @@ template <int N> __device__ __forceinline__ void load_weights(float (&w)[N], con
 // in registers. Memory bounds it, and near that the instructions: at 8191 tokens of 36 rows of 128 bf16 values,
 // normed, with three axes, a row a warp with one value a load took 218 us, chunks without the loads of all steps
 // in flight 75 us, this 45 us (3.4 TB/s; the bytes alone would take 24 us).
-template <typename T, int VE>
+// PART: some values are not turned. They do not go through the product, where x * 1 - inf * 0 would make NaN of what
+// stands beside an infinity. (Asking each lane also where all are turned takes 47 instead of 46 us there, for more
+// spilled registers.)
+template <typename T, int VE, bool PART>
 __global__ void __launch_bounds__(kAppendThreads, 3) append_rows_kernel(const __grid_constant__ AppendArgs a, int lpr,
                                                                        int steps) {
   pdl_wait();
@@ -178,15 +181,21 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_rows_kernel(const __
         }
       }
       if (a.interleaved) {
+        if (!PART || turn_a)
 #pragma unroll
-        for (int e = 0; e < VE / 2; ++e) {
-          const float x0 = fa[2 * e], x1 = fa[2 * e + 1], y0 = fb[2 * e], y1 = fb[2 * e + 1];
-          fa[2 * e] = x0 * cs[e] - x1 * sn[e];
-          fa[2 * e + 1] = x1 * cs[e] + x0 * sn[e];
-          fb[2 * e] = y0 * cs[VE / 2 + e] - y1 * sn[VE / 2 + e];
-          fb[2 * e + 1] = y1 * cs[VE / 2 + e] + y0 * sn[VE / 2 + e];
-        }
-      } else {
+          for (int e = 0; e < VE / 2; ++e) {
+            const float x0 = fa[2 * e], x1 = fa[2 * e + 1];
+            fa[2 * e] = x0 * cs[e] - x1 * sn[e];
+            fa[2 * e + 1] = x1 * cs[e] + x0 * sn[e];
+          }
+        if (!PART || turn_b)
+#pragma unroll
+          for (int e = 0; e < VE / 2; ++e) {
+            const float y0 = fb[2 * e], y1 = fb[2 * e + 1];
+            fb[2 * e] = y0 * cs[VE / 2 + e] - y1 * sn[VE / 2 + e];
+            fb[2 * e + 1] = y1 * cs[VE / 2 + e] + y0 * sn[VE / 2 + e];
+          }
+      } else if (!PART || turn_a) {
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           const float x0 = fa[e], x1 = fb[e];
@@ -194,10 +203,9 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_rows_kernel(const __
           fb[e] = x1 * cs[e] + x0 * sn[e];
         }
       }
-      if (r < turned) {  // values stay as they are, bit for bit
-        xa[k].set(fa);
-        xb[k].set(fb);
-      }
+      // values, and what is neither normed nor turned, stay as they are, bit for bit
+      if (r < turned && (!PART || nw || turn_a)) xa[k].set(fa);
+      if (r < turned && (!PART || nw || turn_b)) xb[k].set(fb);
     }
     if (r >= rows) continue;
     T* y = r < a.heads ? q_out + r * D : r < turned ? k_out + (r - a.heads) * head : v_out + (r - turned) * head;
@@ -596,7 +604,8 @@ tq4_status launch_append_rows(const AppendArgs& a, cudaStream_t st, bool* taken)
   const int most = (int)std::min<int64_t>(kAppendSteps, std::max<int64_t>(1, a.tokens * all / (148 * 16)));
   const int warps = (all + most - 1) / most, steps = (all + warps - 1) / warps;
   const dim3 grid((unsigned)((a.tokens + kWarps - 1) / kWarps), (unsigned)warps);
-  TQ4_CUDA(launch_pdl(append_rows_kernel<T, VE>, grid, dim3(kAppendThreads), 0, st, a, lpr, steps));
+  const auto kern = 2 * a.pairs < a.cache.head_dim ? append_rows_kernel<T, VE, true> : append_rows_kernel<T, VE, false>;
+  TQ4_CUDA(launch_pdl(kern, grid, dim3(kAppendThreads), 0, st, a, lpr, steps));
   return TQ4_OK;
 }
 
