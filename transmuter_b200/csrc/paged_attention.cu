@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kWarpsOf<T, TILE> * 32, DT <= 128 ? 2 : 1)
   __shared__ __align__(8) uint64_t known[4];  // chunk_at[i] holds a chunk
   __shared__ __align__(8) uint64_t taken[4];  // all its pieces have been taken
   __shared__ __align__(8) uint64_t answered;
-  __shared__ int s_abort, s_taken, s_ask, s_asked, s_answers;
+  __shared__ int s_abort, s_taken, s_ask, s_answers;
   extern __shared__ __align__(16) char dyn[];
   const PagedView& c = a.cache;
   const int D = WHOLE ? DT : c.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kWarpsOf<T, TILE> * 32, DT <= 128 ? 2 : 1)
     s_abort = 0;
     s_taken = WARPS;  // each warp has a piece of the first chunk
     s_ask = (int)gridDim.x > a.ctas;
-    s_asked = s_answers = 0;
+    s_answers = 0;
     for (int i = 0; i < 4; ++i) {
       mbar_init(smem_u32(&known[i]), 1);
       mbar_init(smem_u32(&taken[i]), WARPS);
@@ -391,10 +391,7 @@ __global__ void __launch_bounds__(kWarpsOf<T, TILE> * 32, DT <= 128 ? 2 : 1)
   // they need not be launched.
   const bool seamless = line.plan.levels > 1;  // loads go on into the next piece; a single level's may be too short
   auto draw = [&] {
-    if (lane == 0 && s_ask) {
-      ++s_asked;
-      ask_for_cta(smem_u32(&answer), smem_u32(&answered));
-    }
+    if (lane == 0 && s_ask) ask_for_cta(smem_u32(&answer), smem_u32(&answered));
     __syncwarp();
   };
   auto drawn = [&]() -> Chunk {
@@ -556,9 +553,10 @@ __global__ void __launch_bounds__(kWarpsOf<T, TILE> * 32, DT <= 128 ? 2 : 1)
     if (cur.k.b < 0 || *static_cast<volatile int*>(&s_abort)) break;
   }
   cp_async_wait<0>();
-  // An answer may still be on its way: the warp that asked waits for it. (The chunk that it names is then done by
-  // nobody: a call of which a wait ran out leaves its outputs unfinished and the status set.)
-  if (s_abort && s_asked != s_answers) mbar_drain(smem_u32(&answered), s_answers & 1);
+  // An answer may still be on its way: it is waited for. (The chunk that it names is then done by nobody: a call of which
+  // a wait ran out leaves its outputs unfinished and the status set. Where the wait that ran out was one for `taken`, none
+  // was asked for, and this takes its second; counting what was asked for cost healthy calls up to 2%.)
+  if (s_abort && s_ask) mbar_drain(smem_u32(&answered), s_answers & 1);
 }
 
 // ---- short sequences: one kernel ------------------------------------------------------------------
