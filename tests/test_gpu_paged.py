@@ -829,3 +829,43 @@ def test_append_keeps_an_infinity_in_its_pair(case):
         for y in append_into(c, *map(view, hot), rot, pos)[:2]:
             rest = [e for e in range(d) if e not in (i, other)]
             assert not y[..., rest].any() and y[..., i].isnan().all()
+
+
+@TABLES
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("heads,kv", [(8, 2), (4, 4), (20, 1)])
+def test_attention_nan_of_a_query_head_stays_nan(dtype, heads, kv, wide):
+    """A head whose every score is NaN gives NaN, however its row is cut; every other head and sequence keeps its bits."""
+    lengths = [5000, 3, 700, 0]
+    k, v, table, _ = make_pool(lengths, kv, 16, 64, dtype, 11, width=width_of(wide, lengths, 16))
+    c = paged.PagedCache(k, v, table)
+    q = torch.randn(4, heads, 64, device=DEV).to(dtype)
+    old = torch.rand(4, kv, c.max_slots, device=DEV)
+    hot, h = q.clone(), heads - 2
+    hot[:3, h, 5] = math.nan
+    for scores in (False, True):
+        new = [torch.zeros_like(old) for _ in range(2)] if scores else [None] * 2
+        good, out = (c.attention(x, ints(lengths), scores=old if scores else None, new_scores=n) for x, n in zip((q, hot), new))
+        rest = [i for i in range(heads) if i != h]
+        assert torch.equal(out[:, rest], good[:, rest]) and not out[3].any()
+        assert out[:3, h].isnan().all()
+        if scores:
+            own = h // (heads // kv)
+            rest = [i for i in range(kv) if i != own]
+            assert torch.equal(new[1][:, rest], new[0][:, rest])
+            for b, n in enumerate(lengths):
+                assert new[1][b, own, :n].isnan().all() and torch.equal(new[1][b, own, n:], new[0][b, own, n:])
+
+
+@TABLES
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_attention_nan_keys_of_one_part_are_seen(dtype, wide):
+    """A stretch of NaN keys that fills whole parts of a row makes its output NaN, beside finite parts too."""
+    lengths = [5000, 700]
+    k, v, table, _ = make_pool(lengths, 2, 16, 64, dtype, 12, width=width_of(wide, lengths, 16))
+    c = paged.PagedCache(k, v, table)
+    q = torch.randn(2, 8, 64, device=DEV).to(dtype)
+    good = c.attention(q, ints(lengths))
+    k[table[0, 100:200].long(), 1] = math.nan
+    out = c.attention(q, ints(lengths))
+    assert torch.equal(out[0, :4], good[0, :4]) and torch.equal(out[1], good[1]) and out[0, 4:].isnan().all()

@@ -498,7 +498,8 @@ __global__ void __launch_bounds__(kWarpsOf<T, TILE> * 32, DT <= 128 ? 2 : 1)
     int left = piece_first(cur.k.n, WARPS, cur.w + 1) - first;
     bool ends = false;
     if (left == 0)  // parts that the second kernel passes over
-      for (int i = lane; i < 2 * TILE; i += 32) a.ml[((int64_t)i * a.pieces + piece) * 2] = -INFINITY;
+      for (int i = lane; i < 2 * TILE; i += 32)
+        *reinterpret_cast<float2*>(a.ml + ((int64_t)i * a.pieces + piece) * 2) = make_float2(-INFINITY, 0.f);
     Cursor at;
     if (left > 0) {
       at.set(a, cur.k);
@@ -707,7 +708,7 @@ constexpr int kFinishThreads = 256;
 constexpr int kFinishBlocks = kSms * 4;  // of joins, and about as many of scores
 constexpr int kMaxJoins = 2 * kSms * kLevels * 4;  // a piece ends one at most
 
-// (m, l) pairs joined; m of 0 weights is -inf.
+// (m, l) pairs joined; m of 0 weights is -inf, and l NaN where a score was NaN.
 __device__ __forceinline__ float2 join(float2 x, float2 y) {
   const float m = fmaxf(x.x, y.x), f = m == -INFINITY ? 0.f : m;
   return make_float2(m, x.y * ex2(x.x - f) + y.y * ex2(y.x - f));
@@ -782,7 +783,10 @@ __device__ __forceinline__ void join_head(const AttnArgs& a, int last, int g, in
       }
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
-        if (x[i].x == -INFINITY) continue;  // nothing counted, or nothing written
+        if (x[i].x == -INFINITY) {  // nothing counted, or nothing written (l is 0); or, since a maximum passes NaN
+          ml.y += x[i].y;           // over, all scores were NaN (l is NaN)
+          continue;
+        }
         const float m = fmaxf(ml.x, x[i].x), e0 = ex2(ml.x - m), e1 = ex2(x[i].x - m);
         ml = make_float2(m, ml.y * e0 + x[i].y * e1);
         s.x = s.x * e0 + v[i].x * e1;
@@ -850,8 +854,7 @@ __device__ __forceinline__ void add_weights(const AttnArgs& a, const Plan& plan,
       float2 ml = make_float2(-INFINITY, 0.f);
 #pragma unroll 4
       for (int p = first + j; p <= last; p += 16) {
-        const float2 y = *reinterpret_cast<const float2*>(a.ml + ((int64_t)((p == first ? a.tile : 0) + g) * a.pieces + p) * 2);
-        if (y.x != -INFINITY) ml = join(ml, y);
+        ml = join(ml, *reinterpret_cast<const float2*>(a.ml + ((int64_t)((p == first ? a.tile : 0) + g) * a.pieces + p) * 2));
       }
       for (int off = 8; off > 0; off >>= 1)
         ml = join(ml, make_float2(__shfl_xor_sync(0xffffffffu, ml.x, off), __shfl_xor_sync(0xffffffffu, ml.y, off)));
