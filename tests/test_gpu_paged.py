@@ -869,3 +869,33 @@ def test_attention_nan_keys_of_one_part_are_seen(dtype, wide):
     k[table[0, 100:200].long(), 1] = math.nan
     out = c.attention(q, ints(lengths))
     assert torch.equal(out[0, :4], good[0, :4]) and torch.equal(out[1], good[1]) and out[0, 4:].isnan().all()
+
+
+@TABLES
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_of_large_scores(dtype, d, wide):
+    """Scores of 2^26 and more, where f32 cannot tell neighbours 15 apart: the two slots that share the largest have half the
+    weight each, and all products are exact."""
+    n, pair = 300, (20, 250)
+    k, v, table, _ = make_pool([n], 1, 16, d, dtype, 13, width=width_of(wide, [n], 16))
+    c = paged.PagedCache(k, v, table)
+    g = torch.Generator().manual_seed(13)
+    values = torch.randint(-100, 100, (n, d), generator=g).float() * 2
+    for j in range(n):
+        p = table[0, j // 16].item()
+        k[p, 0, j % 16] = 1024.0 if j in pair else 512.0
+        v[p, 0, j % 16] = values[j].to(DEV, dtype)
+    want = ((values[pair[0]] + values[pair[1]]) / 2).to(DEV)
+    for gain in (256.0, 512.0, 1024.0, 4096.0):
+        q = torch.full((1, 4, d), gain, device=DEV, dtype=dtype)
+        scores = torch.zeros(1, 1, c.max_slots, device=DEV)
+        out = c.attention(q, ints([n]), scale=1.0, scores=scores)
+        assert torch.equal(out[0].float(), want.expand(4, d))
+        assert torch.equal(scores[0, 0].nonzero()[:, 0], torch.tensor(pair, device=DEV)) and (scores[0, 0, list(pair)] == 2).all()
+
+
+@TABLES
+@pytest.mark.parametrize("gain,scale", [(40.0, None), (1.0, 0.0), (2.0, -0.3), (1e-3, 2.0), (40.0, 30.0)])
+def test_attention_scales_of_f16(gain, scale, wide):
+    run_attention(F16, 8, 2, 64, 16, [100, 1, 33], 0, True, gain=gain, scale=scale, wide=wide)

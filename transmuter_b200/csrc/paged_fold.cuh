@@ -125,13 +125,15 @@ template <typename T> __host__ __device__ constexpr int row_chunks(int head_dim)
 // heads fills the instruction; K comes by ldmatrix, V by its transposing form, and the weights turn
 // from S^T's layout to P^T's by transposing 8 x 8 blocks between registers. The weights are rounded
 // to the cache's type, once, for that product; l sums them unrounded. For f16 they are scaled by
-// 2^15 (kBias), so that weights down to 2^-29 of the largest keep f16's full precision.
+// 2^15 (kScale) as they are rounded, so that weights down to 2^-29 of the largest keep f16's full precision; o carries
+// that factor until the row's end. (Taken off m instead, the 15 was itself rounded where scores are 2^24 and more, to
+// 16 from 2^26 on, and the largest weight came to 2^16, which f16 does not hold.)
 template <typename T, int DT, int TILE>
 struct MmaFold {
   static constexpr int U = DT == 64 ? 32 : 16;
   static constexpr int NT = TILE / 8;  // column blocks of heads
   static constexpr int KS = DT / 16;   // 16-value steps of a row
-  static constexpr float kBias = std::is_same_v<T, __half> ? 15.f : 0.f;
+  static constexpr float kScale = std::is_same_v<T, __half> ? 32768.f : 1.f;
   uint32_t qf[NT][KS][2];
   float o[NT][KS][4];
   float m[NT][2], l[NT][2];  // heads 2 * (lane % 4) + {0, 1} of each block
@@ -231,7 +233,7 @@ struct MmaFold {
 #pragma unroll
         for (int t = 1; t < U / 16; ++t) mx[j] = fmaxf(mx[j], fmaxf(s[t][n][j], s[t][n][j + 2]));
         for (int off = 4; off < 32; off <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], off));
-        mx[j] = fmaxf(m[n][j], mx[j] - kBias);
+        mx[j] = fmaxf(m[n][j], mx[j]);
         f[j] = mx[j] == -INFINITY ? 0.f : mx[j];  // nothing counted so far: every weight is 0
         moved = moved || mx[j] != m[n][j];
       }
@@ -256,8 +258,8 @@ struct MmaFold {
           p[i] = ex2(s[t][n][i] - f[i & 1]);
           l[n][i & 1] += p[i];
         }
-        pf[t][n][0] = transpose8x8(pack2<T>(p[0], p[1]));
-        pf[t][n][1] = transpose8x8(pack2<T>(p[2], p[3]));
+        pf[t][n][0] = transpose8x8(pack2<T>(p[0] * kScale, p[1] * kScale));
+        pf[t][n][1] = transpose8x8(pack2<T>(p[2] * kScale, p[3] * kScale));
       }
     }
 #pragma unroll
@@ -276,6 +278,7 @@ struct MmaFold {
   // null) o to part[G][pieces][D] and m, l to ml[G][pieces][2].
   __device__ __forceinline__ void end(T* out, float* part, float* ml, int64_t pieces, int G, int D) {
     const int lane = threadIdx.x & 31;
+    constexpr float kOnce = 1.f / kScale;  // a power of two: exact
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -292,11 +295,11 @@ struct MmaFold {
         for (int k = 0; k < KS; ++k) {
           const int d = k * 16 + (lane >> 2);
           if (out) {
-            if (d < D) out[g * D + d] = from_f32<T>(o[n][k][j] * inv);
-            if (d + 8 < D) out[g * D + d + 8] = from_f32<T>(o[n][k][j + 2] * inv);
+            if (d < D) out[g * D + d] = from_f32<T>(o[n][k][j] * (inv * kOnce));
+            if (d + 8 < D) out[g * D + d + 8] = from_f32<T>(o[n][k][j + 2] * (inv * kOnce));
           } else {
-            if (d < D) to[d] = o[n][k][j];
-            if (d + 8 < D) to[d + 8] = o[n][k][j + 2];
+            if (d < D) to[d] = o[n][k][j] * kOnce;
+            if (d + 8 < D) to[d + 8] = o[n][k][j + 2] * kOnce;
           }
         }
       }
