@@ -899,3 +899,18 @@ def test_attention_of_large_scores(dtype, d, wide):
 @pytest.mark.parametrize("gain,scale", [(40.0, None), (1.0, 0.0), (2.0, -0.3), (1e-3, 2.0), (40.0, 30.0)])
 def test_attention_scales_of_f16(gain, scale, wide):
     run_attention(F16, 8, 2, 64, 16, [100, 1, 33], 0, True, gain=gain, scale=scale, wide=wide)
+
+
+# ---- the edges of the arguments -------------------------------------------------------------------
+
+def test_calls_without_tokens_or_sequences():
+    c = simple_cache(BF16)
+    q, k = torch.zeros(0, 4, 64, device=DEV, dtype=BF16), torch.zeros(0, 2, 64, device=DEV, dtype=BF16)
+    none = ints([])
+    ang = torch.randn(4, 32, device=DEV)
+    for rot in (None, paged.Rotary(ang.cos(), ang.sin())):
+        assert c.append(q, k, k, none, none, none, rot).shape == (0, 4, 64)
+        assert c.append(None, k, k, none, none, none, rot) is None
+    assert c.attention(q, none).shape == (0, 4, 64)
+    kept, lengths, _ = c.evict(none, torch.zeros(0, 2, c.max_slots, device=DEV), 2, 1, torch.zeros(0, 1, dtype=torch.int32, device=DEV))
+    assert kept.shape == (0, 2, 2) and lengths.shape == (0,)

@@ -157,6 +157,16 @@ def test_empty_calls_are_done(cache):
     assert lib.tq4_paged_evict(cache, X, 0, Y, 8, 2, Z, 2, P(8 << 32), W, None, 0, None) == 0
 
 
+def test_empty_calls_take_the_null_addresses_of_empty_tensors(cache):
+    lib = _lib.load()
+    r = rotary()
+    for heads, rot in ((4, None), (4, ctypes.byref(r)), (0, None)):
+        assert lib.tq4_paged_append(cache, None, 256, None, 128, None, 128, heads, 0, None, None, None, rot, None, None) == 0
+    assert lib.tq4_paged_attention(cache, None, 256, 4, None, 0, 1.0, 0, None, None, None, None, 0, None) == 0
+    assert lib.tq4_paged_evict(cache, None, 0, None, 8, 2, None, 2, None, None, None, 0, None) == 0
+    assert lib.tq4_paged_append(cache, None, 256, None, 128, None, 128, -1, 0, None, None, None, None, None, None) == 1
+
+
 def test_python_side_refuses_cpu_tensors():
     pages = torch.zeros(4, 2, 16, 64)
     with pytest.raises(ArgumentError, match="CUDA"):

@@ -743,7 +743,8 @@ tq4_status tq4_paged_append(const tq4_paged* cache, const void* q, int64_t q_str
   }
   const tq4_paged_desc& d = cache->desc;
   const int64_t rows = (int64_t)heads + 2 * (int64_t)d.kv_heads;
-  if (heads < 0 || heads > 65535 || (heads > 0) != (q != nullptr) || (q && !q_out)) {
+  // (an empty tensor's address may be null, queries or not)
+  if (heads < 0 || heads > 65535 || (tokens != 0 && ((heads > 0) != (q != nullptr) || (q && !q_out)))) {
     set_error("tq4_paged_append: q and q_out with 1 to 65535 heads, or neither with heads 0");
     return TQ4_ERR_INVALID_ARGUMENT;
   }
