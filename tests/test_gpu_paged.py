@@ -914,3 +914,19 @@ def test_calls_without_tokens_or_sequences():
     assert c.attention(q, none).shape == (0, 4, 64)
     kept, lengths, _ = c.evict(none, torch.zeros(0, 2, c.max_slots, device=DEV), 2, 1, torch.zeros(0, 1, dtype=torch.int32, device=DEV))
     assert kept.shape == (0, 2, 2) and lengths.shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("n", [40, 9000])
+def test_attention_windows_longer_than_any_sequence(dtype, n):
+    """A window that no sequence reaches is no window, up to the largest number: the same kernels, the same bits."""
+    k, v, table, _ = make_pool([n], 2, 64, 64, dtype, 14)
+    c = paged.PagedCache(k, v, table)
+    q = torch.randn(1, 4, 64, device=DEV).to(dtype)
+    old = torch.rand(1, 2, c.max_slots, device=DEV)
+    want, new = c.attention(q, ints([n])), torch.zeros_like(old)
+    want_s = c.attention(q, ints([n]), scores=old, new_scores=new)
+    for window in (c.max_slots, c.max_slots + 1, 1 << 31, (1 << 63) - 33, (1 << 63) - 1):
+        assert torch.equal(c.attention(q, ints([n]), window=window), want)
+        got = torch.zeros_like(old)
+        assert torch.equal(c.attention(q, ints([n]), window=window, scores=old, new_scores=got), want_s) and torch.equal(got, new)

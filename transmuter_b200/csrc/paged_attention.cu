@@ -1143,6 +1143,7 @@ tq4_status tq4_paged_attention(const tq4_paged* cache, const void* q, int64_t q_
     set_error("tq4_paged_attention: new_scores overlaps scores and is not the same buffer");
     return TQ4_ERR_INVALID_ARGUMENT;
   }
+  if (window >= (int64_t)d.max_pages * d.page_size) window = 0;  // no sequence reaches it
   const Workspace ws = workspace_of(d, heads, batch, scores != nullptr);
   if (workspace_bytes < ws.bytes || !aligned16(workspace) || (ws.bytes > 0 && !workspace)) {
     set_error("tq4_paged_attention: the workspace must be 16-byte aligned and hold %lld bytes, got %lld",
