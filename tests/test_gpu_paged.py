@@ -930,3 +930,127 @@ def test_attention_windows_longer_than_any_sequence(dtype, n):
         assert torch.equal(c.attention(q, ints([n]), window=window), want)
         got = torch.zeros_like(old)
         assert torch.equal(c.attention(q, ints([n]), window=window, scores=old, new_scores=got), want_s) and torch.equal(got, new)
+
+
+# ---- sizes at which the kernels take other paths --------------------------------------------------
+
+# dtype, heads, kv, d, pairs, axes, interleaved, norm, offset of the views: rows in chunks of 16, 8 and 4 bytes and of single
+# values; 36, 40, 15 and 29 rows a token, so that a warp's steps mix queries, keys and values and the last is not full
+PROMPTS = [
+    (BF16, 28, 4, 128, 64, 3, False, True, 0), (F16, 32, 4, 128, 32, 1, True, False, 0), (F32, 9, 3, 128, 64, 3, False, True, 0),
+    (BF16, 28, 4, 72, 36, 3, False, True, 0), (F16, 9, 3, 40, 10, 1, False, True, 0), (BF16, 21, 4, 64, 32, 3, True, True, 2),
+    (F16, 9, 3, 64, 32, 1, False, True, 1), (F32, 21, 4, 256, 6, 2, False, False, 0),
+]
+
+
+@pytest.mark.parametrize("tokens", [33, 700, 2500])
+@pytest.mark.parametrize("case", PROMPTS, ids=str)
+def test_append_prompts(case, tokens):
+    """Prompts of ragged sequences packed one after another with padding between them, in float64 on the GPU; the bounds are
+    the oracle's (oracle/paged.py)."""
+    dtype, heads, kv, d, pairs, axes, interleaved, norm, offset = case
+    ps, gen = 16, torch.Generator().manual_seed(tokens + d)
+    lengths = [tokens // 7, tokens // 2, 1, tokens - tokens // 7 - tokens // 2 - 1]
+    start = [5, 0, 30, 16]
+    need = [-(-(s + n) // ps) for s, n in zip(start, lengths)]
+    order = torch.randperm(sum(need) + 3, generator=gen).int()
+    table = torch.full((4, max(need)), -1, dtype=torch.int32)
+    for s, at in enumerate(np.cumsum([0] + need)[:4]):
+        table[s, :need[s]] = order[at:at + need[s]]
+    table = table.to(DEV)
+    seq = torch.cat([torch.cat([torch.full((n,), s), torch.full((s,), -1)]) for s, n in enumerate(lengths)])
+    slot = torch.cat([torch.cat([torch.arange(n) + start[s], torch.full((s,), -9)]) for s, n in enumerate(lengths)])
+    rows = len(seq)
+    pools = [torch.randn(sum(need) + 3, kv, ps, d, generator=gen).to(DEV, dtype) for _ in range(2)]
+    c = paged.PagedCache(*pools, table)
+    width = (heads + 2 * kv) * d
+    x = torch.randn(rows, width + offset, generator=gen).to(DEV, dtype)[:, offset:].unflatten(1, (-1, d))
+    q, k, v = x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:]
+    positions = torch.randint(0, 4000, (axes, rows), generator=gen).int().to(DEV)
+    ang = torch.arange(4000, dtype=torch.float64)[:, None] * (1e4 ** (-torch.arange(pairs, dtype=torch.float64) / pairs))[None]
+    cos, sin = ang.cos().float().to(DEV), ang.sin().float().to(DEV)
+    axis = torch.arange(pairs, device=DEV) % axes
+    w = [torch.rand(d, generator=gen).add(0.5).to(DEV) if norm else None for _ in range(2)]
+    rot = paged.Rotary(cos, sin, pair_axis=axis.tolist(), interleaved=interleaved, q_weight=w[0], k_weight=w[1], eps=1e-6)
+    want_pools = [p.clone() for p in pools]
+    out = torch.full((rows, heads, d), 3.0, device=DEV, dtype=dtype)
+    c.append(q, k, v, seq.int().to(DEV), slot.int().to(DEV), positions, rot, out=out)
+    j = torch.arange(pairs, device=DEV)
+    one, two = (2 * j, 2 * j + 1) if interleaved else (j, j + pairs)
+    at = positions.long()[axis].T  # [rows, pairs]
+    cs, sn = cos.double()[at, j][:, None], sin.double()[at, j][:, None]
+
+    def check(got, x, w):
+        y = x.double()
+        if w is not None:
+            y = y / (y.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
+        bound = y.abs() * (20 * po.U)
+        a, b = y[..., one], y[..., two]
+        bound[..., one] = bound[..., two] = torch.hypot(a, b) * (20 * po.U)
+        y[..., one], y[..., two] = a * cs[live] - b * sn[live], b * cs[live] + a * sn[live]
+        eps = 0.0 if dtype == F32 else half_step(dtype)
+        tiny = 2.0 ** -25 if dtype == F16 else 0.0
+        assert ((got.double() - y).abs() <= bound * (1 + eps) + y.abs() * eps + tiny).all()
+
+    live = (seq >= 0).to(DEV)
+    check(out[live], q[live], w[0])
+    assert (out[~live] == 3).all()
+    s, r = seq.to(DEV)[live], slot.to(DEV)[live]
+    page, row = table.long()[s, r // ps], r % ps
+    check(pools[0][page, :, row], k[live], w[1])
+    want_pools[0][page, :, row], want_pools[1][page, :, row] = pools[0][page, :, row], v[live]
+    assert torch.equal(want_pools[0], pools[0]) and torch.equal(want_pools[1], pools[1])
+
+
+def kept_of(scores, n, keep, recent):
+    """oracle.paged.keep_slots on the GPU, for finite scores."""
+    if n <= keep:
+        return torch.arange(n, device=DEV)
+    best = scores[:n - recent].sort(descending=True, stable=True).indices[:keep - recent]
+    return torch.cat([best.sort().values, torch.arange(n - recent, n, device=DEV)])
+
+
+@pytest.mark.parametrize("lengths,kv,keep,recent", [
+    ([340001, 12, 340000, 0], 2, 30001, 77),       # clusters of eight, each CTA with more keys than it holds
+    ([20000, 9000, 1, 8999, 20011], 3, 9000, 0),   # clusters of four, some rows without a selection
+    ([41300, 40000] + [100] * 100, 2, 500, 50),    # one CTA a row, with more keys than it holds
+    ([340001], 1, 340000, 339999),                 # one slot goes
+], ids=str)
+def test_evict_wide_tables(lengths, kv, keep, recent):
+    """Sequences over the same pages (the old rows are only read), in tables wide enough for each way that a row's keys are
+    shared out; with few values, so that most scores have equals."""
+    ps, d, count = 128, 4, len(lengths)
+    width, new_width = -(-max(lengths) // ps), -(-keep // ps)
+    old = torch.arange(width * kv * ps, device=DEV, dtype=F32)[:, None].expand(-1, d).reshape(width, kv, ps, d)
+    fresh = torch.zeros(count * new_width, kv, ps, d, device=DEV)
+    pool = torch.cat([old, fresh])
+    table = torch.arange(width, device=DEV).int().expand(count, width).contiguous()
+    new = torch.arange(width, width + count * new_width, device=DEV).int().view(count, new_width)
+    c = paged.PagedCache(pool, -pool, table)
+    scores = torch.randint(0, 400, (count, kv, c.max_slots), device=DEV, generator=torch.Generator(DEV).manual_seed(9)).float()
+    kept, new_len, new_sc = c.evict(ints(lengths), scores, keep, recent, new)
+    assert new_len.tolist() == [min(n, keep) for n in lengths]
+    assert torch.equal(pool[:width], old)
+    for b, n in enumerate(lengths):
+        m = min(n, keep)
+        for h in range(kv):
+            idx = kept_of(scores[b, h], n, keep, recent)
+            assert torch.equal(kept[b, h, :m].long(), idx) and (kept[b, h, m:] == -1).all()
+            assert torch.equal(new_sc[b, h, :m], scores[b, h, idx]) and not new_sc[b, h, m:].any()
+            j = torch.arange(m, device=DEV)
+            for pages, sign in ((pool, 1), (c.v_pages, -1)):
+                assert torch.equal(pages[new[b].long()[j // ps], h, j % ps], sign * old[idx // ps, h, idx % ps])
+
+
+@TABLES
+@pytest.mark.parametrize("dtype,heads,kv", [(F16, 20, 1), (BF16, 96, 2), (F32, 24, 2)])
+def test_attention_of_several_head_tiles_with_and_without_scores(dtype, heads, kv, wide):
+    """Scores may choose another kernel, whose sums run in another order: both within the bounds."""
+    lengths = [200, 1, 90]
+    k, v, table, _ = make_pool(lengths, kv, 16, 64, dtype, 15, width=width_of(wide, lengths, 16))
+    c = paged.PagedCache(k, v, table)
+    q = torch.randn(3, heads, 64, device=DEV).to(dtype)
+    old = torch.rand(3, kv, c.max_slots, device=DEV)
+    new = old.clone()
+    check_attention(c.attention(q, ints(lengths)), None, c, q, lengths, 0, None)
+    check_attention(c.attention(q, ints(lengths), scores=old, new_scores=new), new, c, q, lengths, 0, old)
