@@ -72,16 +72,19 @@ typedef struct {
  * rotation are computed in f32 and rounded once. seq[t] < 0 marks a padding token: nothing is
  * written for it, its row of q_out included. rotary may be NULL (no norm, no rotation;
  * positions unused), and q NULL with heads 0 (only the cache is filled). The (seq, slot) of two
- * tokens of a call must differ: which of the two would remain is not defined. q_out may not
- * overlap q, k or v. */
+ * tokens of a call must differ, and so must the cache rows that they stand for where sequences share
+ * pages: which of the two would remain is not defined. q_out may not overlap q, k or v, and no
+ * input may lie in the cache rows that the call writes. Where nothing is turned and there is no norm,
+ * values are copied bit for bit. */
 tq4_status tq4_paged_append(const tq4_paged* cache, const void* q, int64_t q_stride, const void* k,
                             int64_t k_stride, const void* v, int64_t v_stride, int heads,
                             int64_t tokens, const int32_t* seq, const int32_t* slot,
                             const int32_t* positions, const tq4_rotary* rotary, void* q_out,
                             void* stream);
 
-/* Bytes of workspace that tq4_paged_attention needs for these sizes, whatever the lengths and the window (up to 120 MB,
- * and heads * 4 bytes a slot of the page table's rows with scores; 0 for few short rows without). */
+/* Bytes of workspace that tq4_paged_attention needs for these sizes, whatever the lengths and the window: at most 119 MB
+ * and batch * (heads + 1) * 8 bytes, and with scores heads * 4 bytes more a slot of the page table's first batch rows,
+ * in use or not (64 rows of 131072 slots and 32 heads: 1.07 GB). 0 for few short rows without scores. */
 tq4_status tq4_paged_attention_workspace(const tq4_paged* cache, int heads, int64_t batch,
                                          int with_scores, int64_t* bytes);
 
@@ -89,15 +92,19 @@ tq4_status tq4_paged_attention_workspace(const tq4_paged* cache, int heads, int6
  *   out[b][h] = sum_j softmax_j(scale * q[b][h] . K[j]) V[j],  lengths[b] - window <= j < lengths[b]
  * over the rows of KV head h / (heads / kv_heads) of sequence b = row b of the page table, the new
  * token's own row among them (append it first). window = 0 attends to the whole sequence. A
- * sequence of length 0 gives zeros, and so does a head whose every score is -inf. q is [batch][heads][head_dim], rows q_stride values apart; out
- * is dense and may not overlap q. heads is any multiple of kv_heads.
+ * sequence of length 0 gives zeros, and so does a head whose every score is -inf; a NaN among a head's scores gives NaN.
+ * q is [batch][heads][head_dim], rows q_stride values apart; out is dense and may not overlap q, nor any other buffer of
+ * the call. heads is any multiple of kv_heads.
  * With scores and new_scores (f32 [batch][kv_heads][max_pages * page_size], both or neither; they
  * may be the same buffer), the softmax weights that eviction goes by are accumulated: slot j of
  * new_scores is that of scores plus the sum over the KV head's query heads of slot j's weight, and
  * slots at and behind lengths[b] are left as they were.
  * workspace: 16-byte aligned device memory that this call has to itself until it has run (NULL where
- * 0 bytes are needed); what it held before does not matter. Sums, maxima and outputs are accumulated in f32 and in an order that
- * depends on the lengths alone: equal calls give equal bits. */
+ * 0 bytes are needed); what it held before does not matter.
+ * Sums, maxima and outputs are accumulated in f32. Over a 16-bit cache each softmax weight is rounded once to the cache's
+ * type before it multiplies its value (f16: scaled by 2^15 first); the weights' sum and the scores take it unrounded. The
+ * order of the sums depends on the sizes, the page table's shape, the window, whether there are scores, and all lengths
+ * of the batch: calls that are equal in these give equal bits, others may differ in the last bits of f32. */
 tq4_status tq4_paged_attention(const tq4_paged* cache, const void* q, int64_t q_stride, int heads,
                                const int32_t* lengths, int64_t batch, float scale, int64_t window,
                                const float* scores, float* new_scores, void* out, void* workspace,

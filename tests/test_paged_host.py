@@ -136,6 +136,20 @@ def test_attention_workspace_holds_the_scores(cache):
     assert lib.tq4_paged_attention_workspace(cache, 4, 3, 1, None) == 1
 
 
+@pytest.mark.parametrize("dtype", [_lib.F32, _lib.F16])
+@pytest.mark.parametrize("d", [8, 72, 128, 256])
+@pytest.mark.parametrize("max_pages", [1, 5000, 1 << 20])
+@pytest.mark.parametrize("seqs,kv,group", [(1, 1, 64), (64, 8, 4), (5000, 2, 16), (7, 64, 1), (3, 1, 5)])
+def test_attention_workspace_is_bounded_as_documented(dtype, d, max_pages, seqs, kv, group):
+    st, h = create(desc(dtype=dtype, d=d, max_pages=max_pages, seqs=seqs, kv=kv))
+    assert st == 0
+    n, heads = ctypes.c_int64(), kv * group
+    for scores in (0, 1):
+        assert _lib.load().tq4_paged_attention_workspace(h, heads, seqs, scores, ctypes.byref(n)) == 0
+        assert 0 <= n.value <= 119e6 + seqs * (heads + 1) * 8 + scores * seqs * heads * max_pages * 16 * 4
+    _lib.load().tq4_paged_destroy(h)
+
+
 @pytest.mark.parametrize("kw,msg", [
     ({"batch": -1}, "sequences"), ({"batch": 5}, "sequences"), ({"keep": 0}, "keep"), ({"keep": 33}, "keep"),
     ({"recent": -1}, "recent"), ({"recent": 9}, "recent"), ({"len": None}, "null"), ({"sc": None}, "null"),

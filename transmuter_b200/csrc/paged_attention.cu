@@ -18,8 +18,8 @@
 //           softmax). A row inside one piece is finished there; of others the parts go to the workspace.
 //           (With the warps of a CTA joined in shared memory at each row's end, that end took 2.2 us, and
 //           four of them a sixth of the kernel's time for 32 sequences of up to 4096 slots.)
-//   finish  joins the parts in the line's order, so that results depend on the lengths alone and not on
-//           who took which chunk, and adds the softmax weights to the scores.
+//   finish  joins the parts in the line's order, so that results depend on the call's sizes and lengths alone and
+//           not on who took which chunk, and adds the softmax weights to the scores.
 #include "paged_fold.cuh"
 
 namespace tq4 {

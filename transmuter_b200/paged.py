@@ -150,7 +150,8 @@ class PagedCache:
     def append(self, q, k, v, seq, slot, positions=None, rotary=None, out=None):
         """Writes the keys and values of new tokens into the cache (token t is slot ``slot[t]`` of
         sequence ``seq[t]``; seq -1 is padding and nothing of it is touched) and returns their queries,
-        both normed and turned by ``rotary`` at ``positions`` (int32 [tokens], or [axes, tokens]).
+        both normed and turned by ``rotary`` at ``positions`` (int32 [tokens], or [axes, tokens]; what no
+        pair turns is copied bit for bit where there is no norm).
         q [tokens, heads, head_dim], or None when only the cache is filled; k and v [tokens, kv_heads,
         head_dim]; views of a merged projection are read in place. ``out`` may not overlap them."""
         device = self.device
@@ -188,7 +189,9 @@ class PagedCache:
     def attention(self, q, lengths, scale=None, window=0, scores=None, new_scores=None, out=None):
         """Attention of one new token of each sequence b < batch over its ``lengths[b]`` slots (int32
         [batch]; the new token's own among them), or the last ``window`` of them: [batch, heads,
-        head_dim]. Length 0 gives zeros; ``scale`` is 1 / sqrt(head_dim) by default. With ``scores``
+        head_dim]. Length 0 gives zeros; ``scale`` is 1 / sqrt(head_dim) by default. Sums are f32; over a
+        16-bit cache each softmax weight is rounded once to its type before it multiplies its value.
+        ``out`` may not overlap another tensor of the call. With ``scores``
         (f32 [batch, kv_heads, max_pages * page_size]) each slot's softmax weights, summed over the
         query heads of a KV head, are added to them: in place, or into ``new_scores``."""
         device = self.device
