@@ -367,7 +367,11 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int64_t b, int h, 
 }
 
 constexpr int kBins = 2048;     // of a pass over 11 bits of the keys
-constexpr int kMaxCluster = 8;  // CTAs of a row (of 131072 slots: 16 take 89 us, 8 take 42 us, 4 about 39 us)
+// CTAs of a row at most. Of one row of 131072 slots the whole call (64 kept) takes 28 us with 8 and 35 with 4, of one of
+// 340000 slots 119 and 214 us. Where the rows are many 4 are as fast or faster (16 rows of 131072 to 16384: 97.8 and 94.0
+// us; 32 rows of 40000 to 64: 34 and 22 us), which the rule in launch_evict does not tell apart; 16 took twice the time
+// of 8 for the selection of 16 rows.
+constexpr int kMaxCluster = 8;
 
 // One cluster per (sequence, KV head): which slots are kept. A CTA has a share of the candidates, in shared memory
 // as keys. The smallest kept key is found by radix selection in three passes of 11, 11 and 10 bits: the
