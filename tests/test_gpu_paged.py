@@ -1054,3 +1054,32 @@ def test_attention_of_several_head_tiles_with_and_without_scores(dtype, heads, k
     new = old.clone()
     check_attention(c.attention(q, ints(lengths)), None, c, q, lengths, 0, None)
     check_attention(c.attention(q, ints(lengths), scores=old, new_scores=new), new, c, q, lengths, 0, old)
+
+
+def test_calls_on_two_streams_at_once():
+    """Eager steps of two caches side by side, without waiting for one another: each gives the bits that it gives alone."""
+    def make(seed, dtype, lengths):
+        k, v, table, new = make_pool(lengths, 2, 16, 64, dtype, seed, width=width_of(True, lengths, 16), fresh=20)
+        c = paged.PagedCache(k, v, table)
+        g = torch.Generator(DEV).manual_seed(seed)
+        q = torch.randn(len(lengths), 8, 64, device=DEV, generator=g).to(dtype)
+        return c, q, ints(lengths), torch.rand(len(lengths), 2, c.max_slots, device=DEV, generator=g), new
+
+    def step(c, q, n, scores, new):
+        s = scores.clone()
+        out = c.attention(q, n, scores=s)
+        return (out, s, *c.evict(n, s, 300, 40, new))
+
+    cases = [make(41, BF16, [4000, 900, 0, 2500]), make(42, F32, [3000, 1, 1700])]
+    alone = [step(*x) for x in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for x, st in zip(cases, streams):
+            with torch.cuda.stream(st):
+                got.append([step(*x) for _ in range(3)])
+        torch.cuda.synchronize()
+        for want, three in zip(alone, got):
+            for one in three:
+                assert all(torch.equal(a, b) for a, b in zip(want, one))
